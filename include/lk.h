@@ -46,6 +46,9 @@ enum {
 #define LK_FMT_PAIR(gate, up) ((int)(gate) | ((int)(up) << 16))
 /* element types (ggml ids where ggml has one) */
 enum { LK_F32 = 0, LK_F16 = 1, LK_BF16 = 30, LK_E4M3 = 1000 };
+/* activation rows in the form a product reads them, as output forms (LK_E4M3: lk_row_scale_f8's rows): lk_quant_q8's
+ * codes and group meta in one buffer, and lk_row_scale_f16's rows */
+enum { LK_Q8_ROWS = 1001, LK_F16_ROWS = 1002 };
 /* GEMM epilogues (gen_gemm.py:535 `mode`): y = acc, y += acc, y = silu(acc_w) * acc_w2. LK_SWIGLU_SORTED (grouped
  * GEMMs only; no counterpart in the reference, whose gate/up gathers token rows inside the GEMM): the swiglu gate/up
  * on activation rows already in bucket order (lk_moe_row_scale_gather's output), read as plain tiles. */
@@ -56,6 +59,9 @@ enum { LK_ORDER_PAIRS = 0, LK_ORDER_SPLIT16 = 1 };
  * gemma4 kit's ffn_act "gelu", make_kernel_tests.py:78-80); gpt-oss swiglu_oai: x = min(g, limit),
  * y = clamp(u, -limit, limit), x * sigmoid(alpha * x) * (y + 1) (llama.cpp ggml_swiglu_oai; alpha 1.702, limit 7) */
 enum { LK_ACT_SILU = 0, LK_ACT_GELU = 1, LK_ACT_SWIGLU_OAI = 2 };
+/* further activations of the epilogue products (lk_mv_q8_ex, lk_gemm_ex): none, max(g, 0), and 0.5 g (1 + erf(g / sqrt 2));
+ * LK_ACT_GELU is the tanh form */
+enum { LK_ACT_NONE = 3, LK_ACT_RELU = 4, LK_ACT_GELU_ERF = 5 };
 
 #define LK_OK 0
 #define LK_EINVAL (-1)       /* unknown format / mode / dtype, bad shape, null pointer */
@@ -97,6 +103,23 @@ int lk_row_scale_f16(int rows, int k, const void* x, int x_dtype, float* scales,
 int lk_row_scale_f8(int rows, int k, const void* x, int x_dtype, float* scales, uint16_t* x16, uint8_t* x8, float* s8,
                     lk_stream_t stream);
 
+/* lk_rms_norm: the residual addition, the RMS norm and the activation producer of the next product in one launch (no
+ * reference counterpart as one kernel; the parts are g_row_scale_f16, its fp8 twin and g_quant_q8 on a norm's output):
+ *   h = x + residual                 in f32; written to `h` (when not NULL) rounded once to r_dtype
+ *   v = h / sqrt(mean(h^2) + eps) * weight      in f32, from the unrounded h
+ *   y = v in `form`:  LK_F32 / LK_F16 / LK_BF16  [rows][k] values, one rounding
+ *                     LK_Q8_ROWS   lk_quant_q8's buffer (rows*k codes, then the group meta), bit for bit what
+ *                                  lk_quant_q8 makes of v; k % 32 == 0; y 16-byte aligned
+ *                     LK_F16_ROWS  lk_row_scale_f16's x16 [rows][k], `scales` [rows][2]; bit for bit what it makes of v
+ *                     LK_E4M3      lk_row_scale_f8's x8 [rows][k], `scales` = its s8 [rows][2]; likewise
+ * x [rows][k] of x_dtype, residual [rows][k] of r_dtype or NULL (then h must be NULL and r_dtype is not read), weight
+ * [k] of w_dtype: each LK_F32, LK_F16 or LK_BF16. h may be the residual's buffer (the stream updated in place) or, of
+ * x_dtype, x's; a plain y may be x's buffer when its type is x_dtype. No other two operands may overlap. Pointers are
+ * aligned to their elements; 16-byte aligned operands with k % 8 == 0 are moved in 16-byte vectors. k <= 32768
+ * (LK_ERANGE beyond). The sum of squares is held in f32: a row whose |h| passes about 1e17 gives zeros. */
+int lk_rms_norm(int rows, int k, const void* x, int x_dtype, const void* residual, int r_dtype, const void* weight,
+                int w_dtype, float eps, void* h, int form, void* y, float* scales, lk_stream_t stream);
+
 /* ---------------------------------------------------------------------------------------------------------------
  * Decode matvec (tokens < 64). Replaces g_mv_{fmt}_k{K}[_t{TG}][_r{R}] and its swiglu pair (gen_llm.py:1159-1378),
  * launch(%n, %tokens, %accumulate, %x, %w [, %w2], %y): y[t][n] (+)= sum_k x[t][k] W[n][k];
@@ -136,6 +159,20 @@ int lk_mv_q8(int fmt, int n, int k, int tokens, int accumulate, const uint8_t* x
  * n, w, y are HOST arrays of nseg entries. */
 int lk_mv_q8_multi(int fmt, int nseg, const int* n, const void* const* w, float* const* y, int k, int tokens,
                    int accumulate, const uint8_t* xq, lk_stream_t stream);
+/* lk_mv_q8_ex: lk_mv_q8 with what a layer applies to the product in its epilogue, in f32 and in this order:
+ *   p[t][n] = sum_k dequant(W)[n][k] * xcode[t][k] * d[t][k/32]
+ *   v = act(p + bias[n])                                 (w2 NULL)
+ *   v = act(p + bias[n]) * (p2 + bias2[n])               (w2 given: gate and up in one launch, one format, [n] rows each;
+ *                                                         LK_ACT_SWIGLU_OAI: its own product form, see above)
+ *   y = v + residual[t][n], rounded once to y_form
+ * act: LK_ACT_NONE, _SILU, _GELU, _GELU_ERF or _RELU; with w2 also _SWIGLU_OAI (alpha, limit). bias, bias2: f32 [n] or
+ * NULL (bias2 only with w2). residual: [tokens][n] of r_dtype (LK_F32, LK_F16, LK_BF16) or NULL. y_form: LK_F32, LK_F16
+ * or LK_BF16, [tokens][n]; or LK_Q8_ROWS, lk_quant_q8's buffer of the tokens x n values (n % 32 == 0, y 16-byte aligned):
+ * the next product's input. y may be the residual's buffer when both have the same type. xq, k and the formats as
+ * lk_mv_q8 (every format with integer codes); w, w2 2-byte aligned. Any tokens >= 0, any n >= 1. */
+int lk_mv_q8_ex(int fmt, int n, int k, int tokens, const uint8_t* xq, const void* w, const void* w2, const float* bias,
+                const float* bias2, int act, float alpha, float limit, const void* residual, int r_dtype, void* y,
+                int y_form, lk_stream_t stream);
 /* lk_mv_q8_fused / lk_mv_q8_fused_multi: g_quant_q8 (gen_llm.py:683-750) and g_mv_{fmt}_q8 (gen_llm.py:1159-1378) of
  * one token in one launch, launch(%n, %accumulate, %x, %w, %y): the activation row x [1][k] (LK_F32 or LK_BF16) is
  * quantised to Q8_1 codes inside the matvec -- each CTA quantises the row into its shared memory, the codes and group
@@ -163,6 +200,16 @@ int lk_mv_q8_fused_multi(int fmt, int nseg, const int* n, const void* const* w, 
  */
 int lk_gemm(int fmt, int mode, int rows, int k, int n, const uint16_t* x16, const float* scales, const void* w,
             const void* w2, float* y, lk_stream_t stream);
+
+/* lk_gemm_ex: the prefill GEMM with the epilogue of lk_mv_q8_ex:
+ *   p[t][n] = scales[t][1] * sum_k x16[t][k] W16[n][k];  v = act(p + bias) or act(p + bias) * (p2 + bias2);  y = v + residual
+ * W16: lk_gemm's f16 staging of every format it takes (one format for w and w2). The sums, bias, activation and residual
+ * are f32; y is rounded once to y_dtype (LK_F32, LK_F16, LK_BF16). act, alpha, limit, biases and residual as lk_mv_q8_ex;
+ * y may be the residual's buffer when both have the same type. x16, scales as lk_gemm (x16 16-byte aligned), k % 64 == 0
+ * and a whole number of the format's blocks; any rows >= 0 and any n >= 1; w, w2 2-byte aligned (ggml MXFP4: any). */
+int lk_gemm_ex(int fmt, int rows, int k, int n, const uint16_t* x16, const float* scales, const void* w, const void* w2,
+               const float* bias, const float* bias2, int act, float alpha, float limit, const void* residual,
+               int r_dtype, void* y, int y_dtype, lk_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------------------------------
  * MXFP4 (split planes) x FP8 GEMM. Replaces g_gemm_mxfp4s_{store,swiglu}_f8_m256_rdna4

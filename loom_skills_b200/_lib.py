@@ -9,10 +9,13 @@ LIB_PATH = os.path.join(HERE, "liblk.so")
 Q4_0, Q4_K, IQ4_NL, MXFP4, MXFP4S = 2, 12, 20, 39, 1039
 Q5_0, Q8_0, Q3_K, Q5_K, Q6_K, IQ4_XS, IQ3_S = 6, 8, 11, 13, 14, 23, 21
 F32, F16, BF16, E4M3 = 0, 1, 30, 1000
+Q8_ROWS, F16_ROWS = 1001, 1002
 STORE, ACC, SWIGLU, SWIGLU_SORTED = 0, 1, 2, 3
 ORDER_PAIRS, ORDER_SPLIT16 = 0, 1
 ACT_SILU, ACT_GELU, ACT_SWIGLU_OAI = 0, 1, 2
-ACT_IDS = {"silu": ACT_SILU, "gelu": ACT_GELU, "swiglu_oai": ACT_SWIGLU_OAI}
+ACT_NONE, ACT_RELU, ACT_GELU_ERF = 3, 4, 5
+ACT_IDS = {"silu": ACT_SILU, "gelu": ACT_GELU, "swiglu_oai": ACT_SWIGLU_OAI, "none": ACT_NONE, "relu": ACT_RELU,
+           "gelu_erf": ACT_GELU_ERF}
 FMT_IDS = {"q4_0": Q4_0, "q4_k": Q4_K, "iq4_nl": IQ4_NL, "mxfp4": MXFP4, "mxfp4s": MXFP4S, "q5_0": Q5_0,
            "q8_0": Q8_0, "q3_k": Q3_K, "q5_k": Q5_K, "q6_k": Q6_K, "iq4_xs": IQ4_XS,
            "iq3_s": IQ3_S}
@@ -75,6 +78,9 @@ SIGNATURES = {
     "lk_moe_gather_rows": (_I, [_I, _I, _I, _I, _P, _P, _P, _I, _P, _P, _P]),
     "lk_moe_ffn_decode_q8": (_I, [_I, _I, _I, _I, _I, _I, _I, _I, _F, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P, _I,
                                   _F, _F, _P, _P, _P, _P, _I, _P, _P]),
+    "lk_rms_norm": (_I, [_I, _I, _P, _I, _P, _I, _P, _I, _F, _P, _I, _P, _P, _P]),
+    "lk_mv_q8_ex": (_I, [_I, _I, _I, _I, _P, _P, _P, _P, _P, _I, _F, _F, _P, _I, _P, _I, _P]),
+    "lk_gemm_ex": (_I, [_I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _I, _F, _F, _P, _I, _P, _I, _P]),
     "lk_moe_shared_gate": (_I, [_I, _I, _P, _P, _I, _P, _P]),
     "lk_moe_combine_gated": (_I, [_I, _I, _I, _P, _P, _P, _P, _P]),
     "lk_moe_combine_sorted_gated": (_I, [_I, _I, _I, _I, _P, _P, _P, _P, _P, _P]),

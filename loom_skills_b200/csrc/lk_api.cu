@@ -1,6 +1,7 @@
 // The C ABI of liblk: host-side validation, then the kernel launchers. See include/lk.h for the contract of each
 // entry point and the reference interface it replaces.
 #include "lk_common.cuh"
+#include "lk_epi.cuh"
 #include "lk_formats.cuh"
 #include "lk_internal.h"
 
@@ -32,6 +33,20 @@ static int pair_check(int fmt, int64_t k) {
   return LK_OK;
 }
 
+static bool plain_dtype(int dt) { return dt == LK_F32 || dt == LK_F16 || dt == LK_BF16; }
+static uintptr_t elem_bytes(int dt) { return dt == LK_F32 ? 4 : dt == LK_E4M3 ? 1 : 2; }
+
+// the epilogue operands shared by lk_mv_q8_ex and lk_gemm_ex
+static int epilogue_check(const void* w2, const float* bias, const float* bias2, int act, const void* residual,
+                          int r_dtype, const void* y, int y_form) {
+  if (act < LK_ACT_SILU || act > LK_ACT_GELU_ERF || (act == LK_ACT_SWIGLU_OAI && !w2)) return LK_EINVAL;
+  if (bias2 && !w2) return LK_EINVAL;
+  if (residual && !plain_dtype(r_dtype)) return LK_EINVAL;
+  if (residual == y && residual && r_dtype != y_form) return LK_EINVAL;   // in place: one type
+  if (!aligned(bias, 4) || !aligned(bias2, 4) || (residual && !aligned(residual, elem_bytes(r_dtype)))) return LK_EALIGN;
+  if (!aligned(y, y_form == LK_Q8_ROWS ? 16 : elem_bytes(y_form))) return LK_EALIGN;
+  return LK_OK;
+}
 
 extern "C" {
 
@@ -586,6 +601,57 @@ int lk_moe_gather_rows(int rows, int h, int ku, int n_local, const int32_t* orde
   if (!order || !ids || !x || !out) return LK_EINVAL;
   if (!aligned(x, 16) || !aligned(out, 16)) return LK_EALIGN;
   return moe_gather_rows(rows, h, ku, n_local, order, ids, x, x_dtype, out, eid, (cudaStream_t)stream);
+}
+
+int lk_rms_norm(int rows, int k, const void* x, int x_dtype, const void* residual, int r_dtype, const void* weight,
+                int w_dtype, float eps, void* h, int form, void* y, float* scales, lk_stream_t stream) {
+  if (rows < 0 || k <= 0 || !(eps >= 0.0f)) return LK_EINVAL;
+  if (!plain_dtype(x_dtype) || !plain_dtype(w_dtype) || (residual && !plain_dtype(r_dtype))) return LK_EINVAL;
+  const bool scaled = form == LK_F16_ROWS || form == LK_E4M3;
+  if (!plain_dtype(form) && form != LK_Q8_ROWS && !scaled) return LK_EINVAL;
+  if (form == LK_Q8_ROWS && k % 32) return LK_EINVAL;
+  if (h && !residual) return LK_EINVAL;
+  if (k > 32768) return LK_ERANGE;
+  if (rows == 0) return LK_OK;
+  if (!x || !weight || !y || (scaled && !scales)) return LK_EINVAL;
+  if (h && h == x && r_dtype != x_dtype) return LK_EINVAL;   // in place: one type
+  if (y == x && form != x_dtype) return LK_EINVAL;
+  if ((h && y == h) || (residual && y == residual)) return LK_EINVAL;
+  if (!aligned(x, elem_bytes(x_dtype)) || !aligned(weight, elem_bytes(w_dtype))) return LK_EALIGN;
+  if (residual && (!aligned(residual, elem_bytes(r_dtype)) || !aligned(h, elem_bytes(r_dtype)))) return LK_EALIGN;
+  if (!aligned(y, form == LK_Q8_ROWS ? 16 : elem_bytes(form)) || (scaled && !aligned(scales, 4))) return LK_EALIGN;
+  return rms_norm(rows, k, x, x_dtype, residual, r_dtype, weight, w_dtype, eps, h, form, y, scales,
+                  (cudaStream_t)stream);
+}
+
+int lk_mv_q8_ex(int fmt, int n, int k, int tokens, const uint8_t* xq, const void* w, const void* w2, const float* bias,
+                const float* bias2, int act, float alpha, float limit, const void* residual, int r_dtype, void* y,
+                int y_form, lk_stream_t stream) {
+  if (fmt != LK_Q4_0 && fmt != LK_Q4_K && !mv_q8_generic_format(fmt)) return mv_format(fmt) ? LK_EUNSUPPORTED : LK_EINVAL;
+  if (n <= 0 || k <= 0 || tokens < 0 || k % fmt_qk(fmt)) return LK_EINVAL;
+  if (!plain_dtype(y_form) && y_form != LK_Q8_ROWS) return LK_EINVAL;
+  if (y_form == LK_Q8_ROWS && n % 32) return LK_EINVAL;
+  if (int rc = epilogue_check(w2, bias, bias2, act, residual, r_dtype, y, y_form)) return rc;
+  if (tokens == 0) return LK_OK;
+  if (!xq || !w || !y) return LK_EINVAL;
+  if (!aligned(xq, 16) || !aligned(w, 2) || !aligned(w2, 2)) return LK_EALIGN;
+  const Epilogue e{bias, bias2, residual, r_dtype, act, alpha, limit, y, y_form};
+  return mv_q8_ex(fmt, n, k, tokens, xq, w, w2, e, (cudaStream_t)stream);
+}
+
+int lk_gemm_ex(int fmt, int rows, int k, int n, const uint16_t* x16, const float* scales, const void* w, const void* w2,
+               const float* bias, const float* bias2, int act, float alpha, float limit, const void* residual,
+               int r_dtype, void* y, int y_dtype, lk_stream_t stream) {
+  if (!mv_format(fmt)) return LK_EUNSUPPORTED;
+  if (n <= 0 || k <= 0 || rows < 0 || k % 64 || k % fmt_qk(fmt)) return LK_EINVAL;
+  if (!plain_dtype(y_dtype)) return LK_EINVAL;
+  if (int rc = epilogue_check(w2, bias, bias2, act, residual, r_dtype, y, y_dtype)) return rc;
+  if (rows == 0) return LK_OK;
+  if (!x16 || !scales || !w || !y) return LK_EINVAL;
+  if (!aligned(x16, 16) || !aligned(scales, 4)) return LK_EALIGN;
+  if (fmt != LK_MXFP4 && (!aligned(w, 2) || !aligned(w2, 2))) return LK_EALIGN;
+  const Epilogue e{bias, bias2, residual, r_dtype, act, alpha, limit, y, y_dtype};
+  return gemm_ex(fmt, rows, k, n, x16, scales, w, w2, e, (cudaStream_t)stream);
 }
 
 }  // extern "C"

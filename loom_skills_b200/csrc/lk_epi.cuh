@@ -1,0 +1,55 @@
+// What the epilogue products (lk_mv_q8_ex, lk_gemm_ex) and the fused norm share: element loads and stores of the three
+// value types, and the activations.
+#pragma once
+#include "lk_common.cuh"
+
+namespace lk {
+
+// element i of an array of LK_F32 / LK_F16 / LK_BF16
+LK_DEV float load_elem(const void* p, int dtype, int64_t i) {
+  if (dtype == LK_BF16) return bf2f(static_cast<const uint16_t*>(p)[i]);
+  if (dtype == LK_F16) return h2f(static_cast<const uint16_t*>(p)[i]);
+  return static_cast<const float*>(p)[i];
+}
+// one rounding, to nearest even
+LK_DEV void store_elem(void* p, int dtype, int64_t i, float v) {
+  if (dtype == LK_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else if (dtype == LK_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
+  else static_cast<float*>(p)[i] = v;
+}
+
+// The activation of one product. expf, tanhf and erff (not their approximations): a few instructions per output are
+// nothing next to the product, and f32 outputs keep f32 accuracy.
+LK_DEV float act_one(int act, float g) {
+  switch (act) {
+    case LK_ACT_SILU: return g / (1.0f + expf(-g));
+    case LK_ACT_GELU: return 0.5f * g * (1.0f + tanhf(0.7978845608028654f * fmaf(0.044715f * g, g * g, g)));
+    case LK_ACT_GELU_ERF: return 0.5f * g * (1.0f + erff(g * 0.7071067811865476f));
+    case LK_ACT_RELU: return g < 0.0f ? 0.0f : g;   // keeps a NaN
+  }
+  return g;
+}
+// ... and of a gate / up pair
+LK_DEV float act_pair(int act, float g, float u, float alpha, float limit) {
+  if (act == LK_ACT_SWIGLU_OAI) {
+    // comparisons that keep a NaN, as clamp does
+    const float x = g > limit ? limit : g, y = u > limit ? limit : (u < -limit ? -limit : u);
+    return x / (1.0f + expf(-alpha * x)) * (y + 1.0f);
+  }
+  return act_one(act, g) * u;
+}
+
+// Everything an epilogue product applies to its f32 sums, in this order: + bias, activation (of one product, or of the
+// gate times the up product), + residual, one rounding to the output's type.
+struct Epilogue {
+  const float* bias;    // [n] or null
+  const float* bias2;   // [n] of the up product, or null
+  const void* res;      // [rows][n] of res_dtype, or null; may be y
+  int res_dtype;
+  int act;
+  float alpha, limit;
+  void* y;              // [rows][n] of y_form; LK_Q8_ROWS: lk_quant_q8's buffer for rows rows of n values
+  int y_form;
+};
+
+}  // namespace lk

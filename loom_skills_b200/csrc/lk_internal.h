@@ -152,6 +152,15 @@ struct MoeFfnQ8 {
 };
 int moe_ffn_decode_q8(int fmt, const MoeFfnQ8& p, cudaStream_t s);
 
+// the fused norm (lk_norm.cu) and the epilogue products (lk_mvx.cu, lk_gemmx.cu; Epilogue: lk_epi.cuh)
+struct Epilogue;
+int rms_norm(int rows, int k, const void* x, int x_dtype, const void* res, int res_dtype, const void* weight,
+             int w_dtype, float eps, void* h, int form, void* y, float* scales, cudaStream_t s);
+int mv_q8_ex(int fmt, int n, int k, int tokens, const uint8_t* xq, const void* w, const void* w2, const Epilogue& e,
+             cudaStream_t s);
+int gemm_ex(int fmt, int rows, int k, int n, const uint16_t* x16, const float* scales, const void* w, const void* w2,
+            const Epilogue& e, cudaStream_t s);
+
 // device status words of the kernel files (bit 0: a bounded wait gave up)
 unsigned int status_q8(bool clear);
 unsigned int status_mv(bool clear);

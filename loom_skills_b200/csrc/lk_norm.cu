@@ -1,0 +1,304 @@
+// Residual addition, RMS norm and the activation format of the next product in one pass over the row.
+//
+//   h = x + residual                       (f32; stored rounded once to the residual's type)
+//   v = h * rstd * weight,  rstd = 1 / sqrt(mean(h^2) + eps)     (f32, from the unrounded h)
+//   y = v rounded to f32 / f16 / bf16, or the codes lk_quant_q8, lk_row_scale_f16 or lk_row_scale_f8 make of v
+//
+// One CTA per row. Thread t holds the 8-value vectors t, t + T, ... of the row in registers from the first load to the
+// last store, so x and the residual are read once and h and y written once; the only exchanges are the sum of squares
+// (and for the row-scaled forms the row's maximum) through warp shuffles and one shared array. Bound by HBM at many rows
+// and by launch and load latency at few.
+#include "lk_common.cuh"
+#include "lk_epi.cuh"
+#include "lk_internal.h"
+
+namespace lk {
+namespace {
+
+constexpr int kVec = 8;             // values per vector
+constexpr int kNormMaxThreads = 1024;
+
+LK_DEV void nm_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+LK_DEV void nm_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// 8 consecutive values (16-byte aligned)
+LK_DEV void load_vec(const void* p, int dtype, int64_t off, float (&v)[kVec]) {
+  if (dtype == LK_F32) {
+    const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + off);
+    const float4 a = q[0], b = q[1];
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    return;
+  }
+  const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + off);
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (dtype == LK_BF16) {
+      v[2 * j] = __uint_as_float(w[j] << 16);
+      v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+      v[2 * j] = f.x;
+      v[2 * j + 1] = f.y;
+    }
+  }
+}
+LK_DEV void store_vec(void* p, int dtype, int64_t off, const float (&v)[kVec]) {
+  if (dtype == LK_F32) {
+    float4* q = reinterpret_cast<float4*>(static_cast<float*>(p) + off);
+    q[0] = make_float4(v[0], v[1], v[2], v[3]);
+    q[1] = make_float4(v[4], v[5], v[6], v[7]);
+    return;
+  }
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (dtype == LK_BF16) {
+      const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+      w[j] = *reinterpret_cast<const uint32_t*>(&b);
+    } else {
+      const __half2 b = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+      w[j] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+  }
+  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + off) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+struct NormArgs {
+  int k;
+  const void* x;
+  int x_dtype;
+  const void* res;
+  int res_dtype;
+  const void* weight;
+  int w_dtype;
+  float eps;
+  void* h;         // of res_dtype, or null
+  void* y;
+  float* scales;   // row forms: [rows][2]
+  int rows;
+};
+
+// FORM: LK_F32 (any plain type, y_dtype at run time), LK_Q8_ROWS, LK_F16_ROWS or LK_E4M3.
+// VEC: rows of whole 16-byte aligned vectors. Otherwise elements are moved one by one: element u * 8 + j of a thread is
+// t + (8 u + j) T, so a warp still touches consecutive addresses -- except for the q8 form, whose 32-value groups stay
+// in four neighbouring lanes.
+template <int FORM, bool VEC, int NV>
+__global__ void __launch_bounds__(kNormMaxThreads) k_rms_norm(const NormArgs p, int y_dtype) {
+  __shared__ float red[2][32];
+  const int t = threadIdx.x, T = blockDim.x, lane = t & 31, warp = t >> 5, nwarps = T >> 5;
+  const int64_t row = blockIdx.x;
+  const int64_t base = row * p.k;
+  constexpr bool kRuns = VEC || FORM == LK_Q8_ROWS;   // a thread's 8 values are consecutive
+  auto at = [&](int u, int j) { return kRuns ? kVec * (t + u * T) + j : t + (kVec * u + j) * T; };
+
+  nm_launch();
+  nm_wait();
+  float v[NV][kVec];
+  float ss = 0.0f;
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+    if (VEC) {
+      const bool in = at(u, 0) < p.k;
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) v[u][j] = 0.0f;
+      if (in) load_vec(p.x, p.x_dtype, base + at(u, 0), v[u]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) v[u][j] = at(u, j) < p.k ? load_elem(p.x, p.x_dtype, base + at(u, j)) : 0.0f;
+    }
+  }
+  if (p.res) {
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      if (VEC) {
+        if (at(u, 0) < p.k) {
+          float r[kVec];
+          load_vec(p.res, p.res_dtype, base + at(u, 0), r);
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) v[u][j] += r[j];
+          if (p.h) store_vec(p.h, p.res_dtype, base + at(u, 0), v[u]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j)
+          if (at(u, j) < p.k) {
+            v[u][j] += load_elem(p.res, p.res_dtype, base + at(u, j));
+            if (p.h) store_elem(p.h, p.res_dtype, base + at(u, j), v[u][j]);
+          }
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < NV; ++u)
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) ss = fmaf(v[u][j], v[u][j], ss);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+  if (lane == 0) red[0][warp] = ss;
+  __syncthreads();
+  ss = lane < nwarps ? red[0][lane] : 0.0f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+  const float rstd = 1.0f / sqrtf(ss / float(p.k) + p.eps);
+
+  float amax = 0.0f;
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+    if (VEC) {
+      if (at(u, 0) < p.k) {
+        float w[kVec];
+        load_vec(p.weight, p.w_dtype, at(u, 0), w);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) v[u][j] = v[u][j] * rstd * w[j];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kVec; ++j)
+        if (at(u, j) < p.k) v[u][j] = v[u][j] * rstd * load_elem(p.weight, p.w_dtype, at(u, j));
+    }
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) amax = fmaxf(amax, fabsf(v[u][j]));
+  }
+
+  if (FORM == LK_F32) {
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      if (VEC) {
+        if (at(u, 0) < p.k) store_vec(p.y, y_dtype, base + at(u, 0), v[u]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j)
+          if (at(u, j) < p.k) store_elem(p.y, y_dtype, base + at(u, j), v[u][j]);
+      }
+    }
+  } else if (FORM == LK_Q8_ROWS) {
+    // k_quant_q8's rounding of each 32-value group, whose values are in four neighbouring lanes
+    int8_t* codes = static_cast<int8_t*>(p.y) + base;
+    float2* meta = reinterpret_cast<float2*>(static_cast<uint8_t*>(p.y) + int64_t(p.rows) * p.k) + row * (p.k / 32);
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      float gmax = fabsf(v[u][0]);   // not from 0: a group of NaN keeps its NaN scale, as k_quant_q8's does
+#pragma unroll
+      for (int j = 1; j < kVec; ++j) gmax = fmaxf(gmax, fabsf(v[u][j]));
+      gmax = fmaxf(gmax, __shfl_xor_sync(0xFFFFFFFFu, gmax, 1));
+      gmax = fmaxf(gmax, __shfl_xor_sync(0xFFFFFFFFu, gmax, 2));
+      const float d = gmax / 127.0f;
+      uint32_t w[2] = {0u, 0u};
+      int sum = 0;
+      if (gmax > 0.0f) {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+          const int q = int8_t(int(roundf(v[u][j] / d)));
+          sum += q;
+          w[j >> 2] |= (uint32_t(q) & 255u) << (8 * (j & 3));
+        }
+      }
+      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
+      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
+      const int e = at(u, 0);
+      if (e < p.k) {
+        *reinterpret_cast<uint2*>(codes + e) = make_uint2(w[0], w[1]);
+        if ((lane & 3) == 0) meta[e / 32] = make_float2(__half2float(__float2half_rn(d)), float(sum));
+      }
+    }
+  } else {
+    // lk_row_scale_f16 / lk_row_scale_f8's exponents from the row's maximum
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
+    if (lane == 0) red[1][warp] = amax;
+    __syncthreads();
+    amax = lane < nwarps ? red[1][lane] : 0.0f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
+    const int biased = int((__float_as_uint(amax) >> 23) & 255);
+    float s, inv;
+    if (FORM == LK_F16_ROWS) {
+      const int e = min(max(biased - 127 - 13, 0), 100);
+      s = __uint_as_float(uint32_t(127 - e) << 23);
+      inv = __uint_as_float(uint32_t(127 + e) << 23);
+    } else {
+      s = __uint_as_float(uint32_t(min(max(261 - biased, 1), 254)) << 23);
+      inv = __uint_as_float(uint32_t(min(max(biased - 15, 1), 254)) << 23);
+    }
+    if (t == 0) {
+      p.scales[2 * row] = s;
+      p.scales[2 * row + 1] = inv;
+    }
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) v[u][j] *= s;
+      if (FORM == LK_F16_ROWS) {
+        if (VEC) {
+          if (at(u, 0) < p.k) store_vec(p.y, LK_F16, base + at(u, 0), v[u]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < kVec; ++j)
+            if (at(u, j) < p.k) store_elem(p.y, LK_F16, base + at(u, j), v[u][j]);
+        }
+      } else {
+        uint8_t* y8 = static_cast<uint8_t*>(p.y) + base;
+        if (VEC) {
+          if (at(u, 0) < p.k) {
+            uint32_t q[2] = {0u, 0u};
+#pragma unroll
+            for (int j = 0; j < kVec; j += 2)
+              q[j >> 2] |= uint32_t(__nv_cvt_float2_to_fp8x2(make_float2(v[u][j], v[u][j + 1]), __NV_SATFINITE, __NV_E4M3))
+                           << (8 * (j & 3));
+            *reinterpret_cast<uint2*>(y8 + at(u, 0)) = make_uint2(q[0], q[1]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < kVec; ++j)
+            if (at(u, j) < p.k) y8[at(u, j)] = __nv_cvt_float_to_fp8(v[u][j], __NV_SATFINITE, __NV_E4M3);
+        }
+      }
+    }
+  }
+}
+
+template <int FORM, bool VEC, int NV>
+int launch(const NormArgs& a, int y_dtype, int threads, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.rows, 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, k_rms_norm<FORM, VEC, NV>, a, y_dtype) == cudaSuccess ? LK_OK : LK_ECUDA;
+}
+
+template <int FORM, bool VEC>
+int pick(const NormArgs& a, int y_dtype, cudaStream_t s) {
+  const int nvec = (a.k + kVec - 1) / kVec;
+  const int nv = nvec <= kNormMaxThreads ? 1 : nvec <= 2 * kNormMaxThreads ? 2 : 4;
+  const int threads = ((nvec + nv - 1) / nv + 31) / 32 * 32;
+  if (nv == 1) return launch<FORM, VEC, 1>(a, y_dtype, threads, s);
+  if (nv == 2) return launch<FORM, VEC, 2>(a, y_dtype, threads, s);
+  return launch<FORM, VEC, 4>(a, y_dtype, threads, s);
+}
+
+bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace
+
+int rms_norm(int rows, int k, const void* x, int x_dtype, const void* res, int res_dtype, const void* weight,
+             int w_dtype, float eps, void* h, int form, void* y, float* scales, cudaStream_t s) {
+  const NormArgs a{k, x, x_dtype, res, res_dtype, weight, w_dtype, eps, h, y, scales, rows};
+  // 16-byte vectors of whole rows; e4m3 and q8 rows are stored 8 bytes at a time, which an 8-byte aligned y allows
+  const bool vec = k % kVec == 0 && al16(x) && al16(res) && al16(weight) && al16(h) &&
+                   (form == LK_E4M3 ? (reinterpret_cast<uintptr_t>(y) & 7) == 0 : al16(y));
+  switch (form) {
+    case LK_Q8_ROWS: return vec ? pick<LK_Q8_ROWS, true>(a, 0, s) : pick<LK_Q8_ROWS, false>(a, 0, s);
+    case LK_F16_ROWS: return vec ? pick<LK_F16_ROWS, true>(a, 0, s) : pick<LK_F16_ROWS, false>(a, 0, s);
+    case LK_E4M3: return vec ? pick<LK_E4M3, true>(a, 0, s) : pick<LK_E4M3, false>(a, 0, s);
+  }
+  return vec ? pick<LK_F32, true>(a, form, s) : pick<LK_F32, false>(a, form, s);
+}
+
+}  // namespace lk

@@ -19,6 +19,11 @@ order and meaning follow the reference's kernel launch signatures (paths relativ
   moe_wscale         g_moe_wscale                 gen_moe.py:1010-1045   (%tokens, %ids, %wts, %scale)
   moe_shared_gate    g_moe_shared_gate            gen_moe.py:780-823     (%tokens, %x, %w, %sg)
 
+and, with no single kernel of the reference behind them, what a layer runs around those products: rms_norm (residual
+addition, norm and the next product's activation format in one launch), mv_q8_ex / gemm_ex (the decode and prefill
+products with bias, activation or gate/up pair, residual and output type in their epilogue), ffn (the dense gated block
+made of them).
+
 The MoE expert kernels take the reference's activation choice (act: "silu", "gelu" -- GEGLU --, "swiglu_oai") and
 per-expert output biases (gen_moe.py:958-1007, expert_mv bias=True).
 
@@ -64,6 +69,25 @@ def _cuda(*ts):
     for t in ts:
         if t is not None and not t.is_cuda:
             raise L.LkError("liblk ops take CUDA tensors (there is no CPU path)")
+
+
+def _need(ok, what):
+    if not ok:
+        raise L.LkError(what)
+
+
+def _device(*ts):
+    """The one CUDA device all the given tensors are on."""
+    dev = -1
+    for t in ts:
+        if t is not None:
+            if not t.is_cuda:
+                raise L.LkError("liblk ops take CUDA tensors (there is no CPU path)")
+            d = t.get_device()
+            if dev >= 0 and d != dev:
+                raise L.LkError("the tensors are on different devices")
+            dev = d
+    return dev
 
 
 def row_bytes(fmt, k):
@@ -640,3 +664,161 @@ def mv_q8_fused_multi(fmt, ws, x, ns, k, ys=None, accumulate=False):
     L.check(L.load().lk_mv_q8_fused_multi(_fmt(fmt), g, n_arr, w_arr, y_arr, k, 1 if accumulate else 0, _ptr(x),
                                           _DT[x.dtype], _stream()), "lk_mv_q8_fused_multi")
     return ys
+
+
+_NORM_FORMS = {"f32": L.F32, "f16": L.F16, "bf16": L.BF16, "q8": L.Q8_ROWS, "row_f16": L.F16_ROWS, "row_f8": L.E4M3}
+_PLAIN = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def rms_norm(x, weight, eps=1e-6, residual=None, form="bf16", h=None, y=None):
+    """lk_rms_norm: h = x + residual, v = h / sqrt(mean(h^2) + eps) * weight, written as `form`:
+    "f32" / "f16" / "bf16" -> [rows][k]; "q8" -> quant_q8's buffer; "row_f16" -> (x16, scales); "row_f8" -> (x8, s8).
+    x, residual [rows][k] and weight [k] are f32, f16 or bf16, each its own. Returns the output; with a residual,
+    (the output, h) -- h the new residual stream in the residual's type, written to `h` when given (which may be
+    `residual` itself, updated in place). y: the output buffer of a plain or q8 form, when given."""
+    dev = _device(x, weight, residual, h, y)
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return rms_norm(x, weight, eps, residual, form, h, y)
+    _need(form in _NORM_FORMS, f"rms_norm: unknown form {form!r}")
+    _need(x.dim() == 2 and weight.numel() == x.shape[1], "rms_norm: x is [rows][k] and weight [k]")
+    _need(x.dtype in _DT and weight.dtype in _DT, "rms_norm: f32, f16 or bf16 operands")
+    rows, k = x.shape
+    x = x.contiguous()
+    weight = weight.contiguous()
+    rdt = L.F32
+    if residual is not None:
+        _need(residual.shape == x.shape and residual.dtype in _DT, "rms_norm: residual is [rows][k], f32, f16 or bf16")
+        rdt = _DT[residual.dtype]
+        if h is None:
+            h = torch.empty_like(residual, memory_format=torch.contiguous_format)
+        _need(h.shape == x.shape and h.dtype == residual.dtype and h.is_contiguous(),
+              "rms_norm: h is contiguous, of the residual's shape and type")
+        residual = residual.contiguous()
+    else:
+        _need(h is None, "rms_norm: h without a residual")
+    fid = _NORM_FORMS[form]
+    scales = None
+    if y is not None:
+        _need(form in _PLAIN or form == "q8", "rms_norm: y is for the plain and q8 forms")
+        _need(y.is_contiguous() and (y.shape == x.shape and y.dtype == _PLAIN[form] if form in _PLAIN else
+                                     y.dtype == torch.uint8 and y.numel() >= rows * k + rows * (k // 32) * 8),
+              "rms_norm: y does not fit the form")
+    elif form == "q8":
+        y = torch.empty(rows * k + rows * (k // 32) * 8, dtype=torch.uint8, device=x.device)
+    elif form in _PLAIN:
+        y = torch.empty(rows, k, dtype=_PLAIN[form], device=x.device)
+    else:
+        y = torch.empty(rows, k, dtype=torch.float16 if form == "row_f16" else torch.uint8, device=x.device)
+        scales = torch.empty(rows, 2, dtype=torch.float32, device=x.device)
+    L.check(L.load().lk_rms_norm(rows, k, _ptr(x), _DT[x.dtype], _ptr(residual), rdt, _ptr(weight),
+                                 _DT[weight.dtype], eps, _ptr(h), fid, _ptr(y), _ptr(scales), _stream()),
+            "lk_rms_norm")
+    out = y if scales is None else (y, scales)
+    return out if h is None else (out, h)
+
+
+def _epilogue(name, fmt, w, w2, bias, bias2, act, residual, tokens, n, k, out_dtype, y):
+    """What mv_q8_ex and gemm_ex share: the operands checked and made contiguous, the output buffer, the ids."""
+    rb = row_bytes(fmt, k)
+    _need(rb > 0, f"{name}: k is not a whole number of the format's blocks")
+    for t in (w, w2):
+        _need(t is None or (t.is_contiguous() and t.numel() * t.element_size() >= n * rb),
+              f"{name}: a weight holds fewer than n rows, or is not contiguous")
+    for b in (bias, bias2):
+        _need(b is None or b.numel() == n, f"{name}: a bias holds n values")
+    act = _act(act if act is not None else "none" if w2 is None else "silu")
+    rdt = L.F32
+    if residual is not None:
+        _need(residual.shape == (tokens, n) and residual.dtype in _DT,
+              f"{name}: residual is [tokens][n], f32, f16 or bf16")
+        rdt = _DT[residual.dtype]
+        residual = residual.contiguous()
+    if out_dtype == "q8":
+        form, size = L.Q8_ROWS, tokens * n + tokens * (n // 32) * 8
+        _need(n % 32 == 0, f"{name}: the q8 output needs n % 32 == 0")
+        if y is None:
+            y = torch.empty(size, dtype=torch.uint8, device=w.device)
+        _need(y.dtype == torch.uint8 and y.is_contiguous() and y.numel() >= size, f"{name}: y is a q8 buffer")
+    else:
+        _need(out_dtype in _DT, f"{name}: out_dtype is f32, f16, bf16 or 'q8'")
+        form = _DT[out_dtype]
+        if y is None:
+            y = torch.empty(tokens, n, dtype=out_dtype, device=w.device)
+        _need(y.shape == (tokens, n) and y.dtype == out_dtype and y.is_contiguous(),
+              f"{name}: y is contiguous, [tokens][n] of out_dtype")
+    return _f32c(bias), _f32c(bias2), act, residual, rdt, form, y
+
+
+def mv_q8_ex(fmt, w, xq, n, k, tokens, w2=None, bias=None, bias2=None, act=None, residual=None,
+             out_dtype=torch.float32, y=None, alpha=1.702, limit=7.0):
+    """lk_mv_q8_ex: the decode product on int8 activations (quant_q8's buffer for `tokens` rows) with its epilogue in
+    f32: act(x.W + bias), or with w2 act(x.W + bias) * (x.W2 + bias2), then + residual, rounded once to out_dtype
+    (f32, f16, bf16; "q8": quant_q8's buffer of the [tokens][n] result, the next product's input). act: "none" (the
+    default of one weight), "silu" (of a pair), "gelu", "gelu_erf", "relu", for a pair also "swiglu_oai". y may be the
+    residual itself (the stream updated in place)."""
+    dev = _device(w, xq, w2, bias, bias2, residual, y)
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return mv_q8_ex(fmt, w, xq, n, k, tokens, w2, bias, bias2, act, residual, out_dtype, y, alpha, limit)
+    _need(xq.is_contiguous() and xq.numel() * xq.element_size() >= tokens * k + tokens * (k // 32) * 8,
+          "mv_q8_ex: xq holds fewer than `tokens` rows")
+    bias, bias2, act, residual, rdt, form, y = _epilogue("mv_q8_ex", fmt, w, w2, bias, bias2, act, residual, tokens, n,
+                                                         k, out_dtype, y)
+    L.check(L.load().lk_mv_q8_ex(_fmt(fmt), n, k, tokens, _ptr(xq), _ptr(w), _ptr(w2), _ptr(bias), _ptr(bias2), act,
+                                 alpha, limit, _ptr(residual), rdt, _ptr(y), form, _stream()), "lk_mv_q8_ex")
+    return y
+
+
+def gemm_ex(fmt, x16, scales, w, n, w2=None, bias=None, bias2=None, act=None, residual=None, out_dtype=torch.float32,
+            y=None, alpha=1.702, limit=7.0):
+    """lk_gemm_ex: the prefill product of row-scaled f16 activations (row_scale_f16, or rms_norm's "row_f16") with
+    mv_q8_ex's epilogue: act(x.W + bias), or act(x.W + bias) * (x.W2 + bias2), then + residual, rounded once to
+    out_dtype (f32, f16, bf16). y may be the residual itself."""
+    dev = _device(x16, scales, w, w2, bias, bias2, residual, y)
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return gemm_ex(fmt, x16, scales, w, n, w2, bias, bias2, act, residual, out_dtype, y, alpha, limit)
+    _need(x16.dim() == 2 and x16.dtype == torch.float16 and scales.shape == (x16.shape[0], 2)
+          and scales.dtype == torch.float32, "gemm_ex: x16 is [rows][k] f16 and scales [rows][2] f32")
+    _need(out_dtype != "q8", "gemm_ex: out_dtype is f32, f16 or bf16")
+    rows, k = x16.shape
+    x16, scales = x16.contiguous(), scales.contiguous()
+    bias, bias2, act, residual, rdt, form, y = _epilogue("gemm_ex", fmt, w, w2, bias, bias2, act, residual, rows, n, k,
+                                                         out_dtype, y)
+    L.check(L.load().lk_gemm_ex(_fmt(fmt), rows, k, n, _ptr(x16), _ptr(scales), _ptr(w), _ptr(w2), _ptr(bias),
+                                _ptr(bias2), act, alpha, limit, _ptr(residual), rdt, _ptr(y), form, _stream()),
+            "lk_gemm_ex")
+    return y
+
+
+# formats with integer weight codes: the decode products on int8 activations take them
+_Q8_FORMATS = ("q4_0", "q4_k", "q8_0", "q5_0", "q5_k", "q6_k", "iq4_nl", "iq4_xs")
+
+
+def ffn(fmt, x, norm_w, w_gate, w_up, w_down, h, f, residual=None, eps=1e-6, act="silu", b_gate=None, b_up=None,
+        b_down=None, fmt_down=None, prefill=None, alpha=1.702, limit=7.0):
+    """The dense gated FFN block of a pre-norm layer, the counterpart of moe_ffn:
+        s = x + residual;  v = rms_norm(s) * norm_w;  s + Wd (act(Wg v + b_gate) * (Wu v + b_up)) + b_down
+    x [tokens][h] (the block before's output) and residual [tokens][h] (the stream; None: x is the stream), f32, f16 or
+    bf16; returns the new stream [tokens][h] in the stream's type. w_gate, w_up: f rows of h values in fmt; w_down: h
+    rows of f values in fmt_down or fmt. Decode (fewer than 64 tokens, the reference's switch, gen_llm.py:6107, and
+    formats with integer codes): int8 activations, three launches -- norm to q8 codes, gate/up to q8 codes, down onto
+    the stream. Prefill: norm to row-scaled f16, gate/up GEMM, row scale, down GEMM onto the stream; the activations
+    between the two GEMMs are held in the stream's type. `prefill` forces either path."""
+    tokens = x.shape[0]
+    fd = fmt_down or fmt
+    stream = x if residual is None else residual
+    if prefill is None:
+        prefill = tokens >= 64 or fmt not in _Q8_FORMATS or fd not in _Q8_FORMATS
+    ep = dict(w2=w_up, bias=b_gate, bias2=b_up, act=act, alpha=alpha, limit=limit)
+    form = "row_f16" if prefill else "q8"
+    v, s = rms_norm(x, norm_w, eps, residual=residual, form=form) if residual is not None else \
+        (rms_norm(x, norm_w, eps, form=form), x)
+    if prefill:
+        a = gemm_ex(fmt, v[0], v[1], w_gate, f, out_dtype=torch.bfloat16 if stream.dtype == torch.bfloat16
+                    else torch.float32, **ep)
+        a16, asc = row_scale_f16(a)
+        return gemm_ex(fd, a16, asc, w_down, h, bias=b_down, residual=s, out_dtype=stream.dtype)
+    a = mv_q8_ex(fmt, w_gate, v, f, h, tokens, out_dtype="q8", **ep)
+    return mv_q8_ex(fd, w_down, a, h, f, tokens, bias=b_down, residual=s, out_dtype=stream.dtype)

@@ -1,0 +1,128 @@
+"""The dense gated FFN block (ops.ffn): norm, gate/up and down products onto the residual stream, run together, against
+float64; and the fused norm in front of the framework's other products."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from oracle import epilogue_oracle as E  # noqa: E402
+from oracle import qmm_oracle as O  # noqa: E402
+
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+QUANT = {"q4_0": O.quantize_q4_0, "q4_k": O.quantize_q4_k, "iq4_nl": O.quantize_iq4_nl}
+
+
+@pytest.fixture(scope="module")
+def ops():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    from loom_skills_b200 import ops as _ops
+    return _ops
+
+
+def dev(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def weights(fmt, n, k, seed):
+    return QUANT[fmt]((np.random.default_rng(seed).standard_normal((n, k)) * 0.05).astype(np.float32))
+
+
+def f16_rows(a):
+    x16, sc = O.row_scale_f16(a.astype(np.float32))
+    return x16.astype(np.float64) * sc[:, 1:]
+
+
+def block_ref(fmt, x, r, nw, wg, wu, wd, h, f, act, bg, bu, bd, decode):
+    """float64, with the activations rounded where the path rounds them (codes, or f16 rows) and the weights it
+    multiplies (the exact values, or the GEMM's f16 staging, whose own distance from them is the GEMM's to test)."""
+    s, v = E.rms_norm(x, nw, np.float32(1e-6), r)
+    quantise = (lambda a: O.dequant_q8(*O.quant_q8(a.astype(np.float32)))) if decode else f16_rows
+    value = O.dequant if decode else O.dequant_f16
+    wv = [value(fmt, w, k).astype(np.float64) for w, k in ((wg, h), (wu, h), (wd, f))]
+    v = quantise(v)
+    a = E.act_pair(act, v @ wv[0].T + bg, v @ wv[1].T + bu)
+    return s + quantise(a) @ wv[2].T + bd
+
+
+@pytest.mark.parametrize("fmt", ["q4_0", "q4_k", "iq4_nl"])
+@pytest.mark.parametrize("tokens,prefill", [(1, None), (7, None), (33, False), (64, None), (200, None), (5, True)])
+@pytest.mark.parametrize("dt,act", [("bf16", "silu"), ("f32", "gelu"), ("f32", "swiglu_oai")])
+def test_block(ops, fmt, tokens, prefill, dt, act):
+    h, f = 512, 768
+    rng = np.random.default_rng(tokens)
+    x, r = (dev(rng.standard_normal((tokens, h)).astype(np.float32) * a).to(DT[dt]) for a in (1, 2))
+    nw = rng.uniform(0.5, 1.5, h).astype(np.float32)
+    wg, wu, wd = weights(fmt, f, h, 1), weights(fmt, f, h, 2), weights(fmt, h, f, 3)
+    bg, bu, bd = (rng.standard_normal(m).astype(np.float32) for m in (f, f, h))
+    y = ops.ffn(fmt, x, dev(nw), dev(wg), dev(wu), dev(wd), h, f, residual=r, act=act, b_gate=dev(bg), b_up=dev(bu),
+                b_down=dev(bd), prefill=prefill)
+    assert y.dtype == DT[dt] and y.shape == (tokens, h)
+    decode = prefill is False or (prefill is None and tokens < 64)
+    args = (fmt, x.double().cpu().numpy(), r.double().cpu().numpy(), nw, wg, wu, wd, h, f, act, bg, bu, bd)
+    ref = block_ref(*args, decode)
+    # a code or an f16 that rounds the other way (f32 against f64 near a tie) moves a value by 1/127 of its group's
+    # largest, or 2^-11, for few values: the framework's bar of 1e-3 covers it. A bf16 stream rounds the result, and in
+    # prefill the activations between the GEMMs, by at most 2^-8 each.
+    tol = 1e-3 + {"f32": 0.0, "bf16": 2.0 ** -8}[dt] * (1 if decode else 2)
+    assert O.rel_l2(y.double().cpu().numpy(), ref) <= tol
+    assert ops.device_status() == 0
+
+
+def test_without_a_residual_and_a_wider_down(ops):
+    h, f = 512, 512
+    rng = np.random.default_rng(5)
+    x = dev(rng.standard_normal((3, h)).astype(np.float32))
+    nw = np.ones(h, np.float32)
+    wg, wu, wd = weights("q4_k", f, h, 1), weights("q4_k", f, h, 2), weights("q4_0", h, f, 3)
+    y = ops.ffn("q4_k", x, dev(nw), dev(wg), dev(wu), dev(wd), h, f, fmt_down="q4_0")
+    v = O.dequant_q8(*O.quant_q8(E.rms_norm(x.double().cpu().numpy(), nw, np.float32(1e-6))[1].astype(np.float32)))
+    a = E.act_pair("silu", v @ O.dequant("q4_k", wg, h).T.astype(np.float64), v @ O.dequant("q4_k", wu, h).T)
+    ref = x.double().cpu().numpy() + O.dequant_q8(*O.quant_q8(a.astype(np.float32))) @ O.dequant("q4_0", wd, f).T
+    assert O.rel_l2(y.double().cpu().numpy(), ref) <= 1e-3
+
+
+def test_captured_layers(ops):
+    """Two blocks in one graph, the stream updated between them: replays follow new inputs."""
+    h, f, fmt = 1024, 1024, "q4_k"
+    nw = torch.ones(h, device="cuda")
+    ws = [[dev(weights(fmt, *s, seed + 10 * i)) for seed, s in enumerate(((f, h), (f, h), (h, f)))] for i in range(2)]
+
+    def two(x, r):
+        for w in ws:
+            x = ops.ffn(fmt, x, nw, *w, h, f, residual=r)
+        return x
+
+    for tokens in (1, 9, 100):
+        x, r = (torch.randn(tokens, h, device="cuda").bfloat16() for _ in range(2))
+        want = two(x, r)
+        xs, rs = torch.zeros_like(x), torch.zeros_like(r)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = two(xs, rs)
+        xs.copy_(x)
+        rs.copy_(r)
+        for _ in range(3):
+            g.replay()
+        assert torch.equal(y, want)
+
+
+def test_norm_before_the_other_products(ops):
+    """rms_norm's codes into mv_q8, its f16 rows into gemm, its e4m3 rows into the MXFP4 GEMM: each the product of the
+    framework's own producer run on the f32 norm, bit for bit."""
+    rng = np.random.default_rng(9)
+    h, n = 512, 256
+    x, r = (dev(rng.standard_normal((70, h)).astype(np.float32)) for _ in range(2))
+    nw = dev(rng.uniform(0.5, 1.5, h).astype(np.float32))
+    v, _ = ops.rms_norm(x, nw, residual=r, form="f32")
+    w = dev(weights("q4_k", n, h, 4))
+    q, _ = ops.rms_norm(x[:5], nw, residual=r[:5], form="q8")
+    assert torch.equal(ops.mv_q8("q4_k", w, q, n, h, 5), ops.mv_q8("q4_k", w, ops.quant_q8(v[:5]), n, h, 5))
+    (x16, sc), _ = ops.rms_norm(x, nw, residual=r, form="row_f16")
+    assert torch.equal(ops.gemm("q4_k", "store", x16, sc, w, n), ops.gemm("q4_k", "store", *ops.row_scale_f16(v), w, n))
+    (x8, s8), _ = ops.rms_norm(x, nw, residual=r, form="row_f8")
+    nib = torch.randint(0, 256, (n, h // 2), dtype=torch.uint8, device="cuda")
+    e8 = torch.randint(118, 124, (n, h // 32), dtype=torch.uint8, device="cuda")
+    assert torch.equal(ops.gemm_mxfp4s_f8("store", x8, s8, nib, e8, n),
+                       ops.gemm_mxfp4s_f8("store", *ops.row_scale_f8(v), nib, e8, n))
