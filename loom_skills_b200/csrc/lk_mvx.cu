@@ -7,11 +7,15 @@
 // token as for 8, and the packed 4-bit words are already in its operand order (byte i of a block holds values i and
 // 16 + i: one word gives a thread its low and its high half), so a weight is unpacked once for all tokens of the call.
 //
-// A CTA walks tiles of 32 weight rows (of a pair: 16 gate and 16 up rows) over all of k in stages of 1024 values. A
-// producer warp bulk-copies each row's 16-byte aligned window and the tokens' codes and group meta into a ring; 16
-// consumer warps take a row half and one of 8 k slices of 128 values each, so a warp's f32 sums are 4 per 8 tokens, and
-// meet at the tile's end in shared memory. There every output is finished by one thread, in a fixed order of sums.
-#include <mutex>
+// A CTA walks tiles of 32 weight rows (of a pair: 16 gate and 16 up rows) over all of k in stages. A producer fills a
+// ring; 16 consumer warps take a row half and one of 8 k slices, so a warp's f32 sums are 4 per 8 tokens, and meet at the
+// tile's end in shared memory. There every output is finished by one thread, in a fixed order of sums.
+//
+// Two ways into shared memory. Box form (rows, codes and meta at 16-byte strides): TMA boxes of 128 bytes x 32 rows in
+// the 128-byte swizzle, which puts the 8 rows x 4 words a warp reads at once into 32 banks; the activations stay in
+// shared memory after a CTA's first tile where they leave three stages of weights. Row form (anything else): a bulk copy
+// per row and token into padded slots; a copy costs about 85 clocks whatever its size, which bounds this form.
+#include <cstring>
 
 #include "lk_common.cuh"
 #include "lk_epi.cuh"
@@ -19,33 +23,47 @@
 #include "lk_internal.h"
 
 namespace lk {
+
+int make_map(CUtensorMap* map, const void* base, CUtensorMapDataType dt, int elem_bytes, int64_t rows, int64_t cols,
+             int box_cols, int box_rows, CUtensorMapSwizzle swz);
+
 namespace {
 
 constexpr int kRows = 32;              // weight rows of a tile
 constexpr int kSlices = 8;             // k slices of a stage
-constexpr int kSliceG = 4;             // 32-value groups of a slice
-constexpr int kStageV = kSlices * kSliceG * 32;
 constexpr int kCWarps = 2 * kSlices;   // consumer warps
 constexpr int kThreads = 32 * (1 + kCWarps);
 constexpr int kTokStride = 36;         // floats between tokens of the partial sums: conflict-free stores
 constexpr int kSmemMax = 227 * 1024;
+constexpr int kMaxStages = 8;
 constexpr uint32_t kWaitPolls = 1u << 22;
 
 LK_DEV void mx_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 LK_DEV void mx_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// row slots of the shared stages: 16 bytes past a multiple of 128, so that the 8 rows x 4 words a warp reads at once
-// fall into 32 banks; with room for a window's 15 leading bytes and a realigning load's trailing word
-__host__ __device__ constexpr int slot_of(int bytes) { return (bytes + 32 + 111) / 128 * 128 + 16; }
-__host__ __device__ constexpr int stage_bytes(int fmt) { return kStageV / fmt_qk(fmt) * fmt_block_bytes(fmt); }
-constexpr int kXSlot = slot_of(kStageV), kMetaSlot = slot_of(kStageV / 32 * 8);
-constexpr int slot_bytes(int fmt, int nt) { return kRows * slot_of(stage_bytes(fmt)) + 8 * nt * (kXSlot + kMetaSlot); }
-constexpr int red_bytes(int nt) { return kSlices * 8 * nt * kTokStride * 4; }
-constexpr int kTailBytes = 256 + 16 * 32 * 4;   // barriers; the first tile of a pair of tiles (q8 output of a pair)
-constexpr int stages_of(int fmt, int nt) {
-  const int s = (kSmemMax - red_bytes(nt) - kTailBytes) / slot_bytes(fmt, nt);
-  return s > 8 ? 8 : s;
+// How a call's operands reach shared memory, and its tokens: kBox1 is the box form of one token, whose codes need no
+// swizzle (all rows read the same words) and come by plain bulk copies.
+enum { kRowForm = 0, kBox = 1, kBox1 = 2 };
+// values of a stage: 2048 for up to 8 tokens, else 1024 (the same in every form, so that all sum in the same order)
+__host__ __device__ constexpr int stage_values(int nt) { return nt == 1 ? 2048 : 1024; }
+// packed bytes of a row's stage; 128-byte segments that can hold them wherever they start
+__host__ __device__ constexpr int stage_bytes(int fmt, int v) { return v / fmt_qk(fmt) * fmt_block_bytes(fmt); }
+__host__ __device__ constexpr int segments(int fmt, int v) {
+  return stage_bytes(fmt, v) % 128 == 0 ? stage_bytes(fmt, v) / 128 : (stage_bytes(fmt, v) + 126) / 128 + 1;
 }
+// row form slots: 16 bytes past a multiple of 128, so that 8 rows x 4 words fall into 32 banks; with room for a window's
+// 15 leading bytes and a realigning load's trailing word
+__host__ __device__ constexpr int slot_of(int bytes) { return (bytes + 32 + 111) / 128 * 128 + 16; }
+// weight bytes of a stage in shared memory, and a stage's activations (box forms: multiples of 1024, which the swizzle's
+// pattern is aligned to)
+__host__ __device__ constexpr int w_bytes(int fmt, int form, int v) {
+  return form == kRowForm ? kRows * slot_of(stage_bytes(fmt, v)) : segments(fmt, v) * kRows * 128;
+}
+__host__ __device__ constexpr int x_bytes(int form, int nt, int v) {
+  return form == kRowForm ? 8 * nt * (slot_of(v) + slot_of(v / 4)) : form == kBox1 ? (v + v / 4 + 1023) / 1024 * 1024 : 8 * nt * (v + v / 4);
+}
+constexpr int red_bytes(int nt) { return kSlices * 8 * nt * kTokStride * 4; }
+constexpr int kTailBytes = 256 + 16 * 32 * 4;   // barriers; the first tile of a unit of two (q8 output of a pair)
 
 struct MvxArgs {
   int n, k, tokens;
@@ -56,6 +74,8 @@ struct MvxArgs {
   int64_t rb;
   int units;             // tiles, or pairs of tiles (q8 output of a gate / up pair), of one token tile
   int tiles_per_unit;
+  int stages;            // ring slots
+  int resident;          // the activations of all of k stay in shared memory
   Epilogue e;
 };
 
@@ -73,14 +93,37 @@ LK_DEV uint32_t lds16(uint32_t a) {
   asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
   return v;
 }
-// the word at a 2-byte aligned address (AL: 4-byte aligned)
-template <bool AL>
-LK_DEV uint32_t ldw(uint32_t a) {
-  if (AL) return lds(a);
-  const uint32_t b = a & ~3u;
-  return __funnelshift_r(lds(b), lds(b + 4), (a & 3u) * 8u);
+// Where byte b of a weight row's stage sits in shared memory. Row form: linear from the row's window.
+struct RowAt {
+  uint32_t p;
+  LK_DEV uint32_t operator()(uint32_t b) const { return p + b; }
+};
+// Box form: 128-byte segments, `pitch` bytes apart, of swizzled rows (16-byte chunk c of row r at c ^ (r & 7))
+template <int PITCH>
+struct BoxAt {
+  uint32_t p, off, x;   // the row in segment 0; the stage's first byte in it; (row & 7) << 4
+  LK_DEV uint32_t operator()(uint32_t b) const {
+    b += off;
+    return p + (b >> 7) * PITCH + ((b & 0x7Fu) ^ x);
+  }
+};
+// the word at byte b, 2-byte aligned (AL: known to be 4-byte aligned)
+template <bool AL, class At>
+LK_DEV uint32_t ldw(const At& at, uint32_t b) {
+  if (AL) return lds(at(b));
+  const uint32_t lo = at(b & ~3u), hi = at((b & ~3u) + 4);
+  // the row form's start may itself be off a word: its at() keeps the low bits
+  return __funnelshift_r(lds(lo), lds(hi), (b & 3u) * 8u);
 }
-LK_DEV float lds_f16(uint32_t a) { return h2f(uint16_t(lds16(a))); }
+template <bool AL>
+LK_DEV uint32_t ldw(const RowAt& at, uint32_t b) {
+  const uint32_t a = at(b);
+  if (AL) return lds(a);
+  const uint32_t c = a & ~3u;
+  return __funnelshift_r(lds(c), lds(c + 4), (a & 3u) * 8u);
+}
+template <class At>
+LK_DEV float lds_f16(const At& at, uint32_t b) { return h2f(uint16_t(lds16(at(b)))); }
 
 // One weight row's slice of 4 groups: the packed words a thread (t = lane & 3) contributes to the MMAs. For group j,
 // lo(j) holds the codes of values 4t .. 4t + 3 and hi(j) those of 16 + 4t .. 16 + 4t + 3, one per byte, as UNSIGNED ? u8 :
@@ -91,42 +134,43 @@ struct Slice {
   static constexpr int kQk = fmt_qk(FMT), kBb = fmt_block_bytes(FMT);
   uint32_t r[FMT == LK_Q8_0 || FMT == LK_Q5_0 ? 8 : FMT == LK_Q5_K || FMT == LK_Q6_K ? 6 : 4];
 
-  // p: the row's chunk in shared memory; ks: the slice
-  LK_DEV void load(uint32_t p, int ks, int t) {
+  // at: the row's stage in shared memory; ks: which 128 values of it
+  template <class At>
+  LK_DEV void load(const At& at, int ks, int t) {
     if (kQk == 32) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t b = p + (4 * ks + j) * kBb;
+        const uint32_t b = (4 * ks + j) * kBb;
         if (FMT == LK_Q8_0) {
-          r[2 * j] = ldw<AL>(b + 2 + 4 * t);
-          r[2 * j + 1] = ldw<AL>(b + 18 + 4 * t);
+          r[2 * j] = ldw<AL>(at, b + 2 + 4 * t);
+          r[2 * j + 1] = ldw<AL>(at, b + 18 + 4 * t);
         } else if (FMT == LK_Q5_0) {
-          r[2 * j] = ldw<AL>(b + 6 + 4 * t);
+          r[2 * j] = ldw<AL>(at, b + 6 + 4 * t);
           // bits 4t .. 4t + 3 and 16 + 4t .. of qh, in one word: bits 0-3 and 16-19
-          r[2 * j + 1] = (ldw<AL>(b + 2) >> (4 * t)) & 0x000F000Fu;
+          r[2 * j + 1] = (ldw<AL>(at, b + 2) >> (4 * t)) & 0x000F000Fu;
         } else {
-          r[j] = ldw<AL>(b + 2 + 4 * t);
+          r[j] = ldw<AL>(at, b + 2 + 4 * t);
         }
       }
     } else {
-      const uint32_t b = p + (ks >> 1) * kBb;   // the slice is half a super-block: groups 4 h .. 4 h + 3
+      const uint32_t b = (ks >> 1) * kBb;   // the slice is half a super-block: groups 4 h .. 4 h + 3
       const int h = ks & 1;
       if (FMT == LK_Q4_K) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = ldw<AL>(b + 16 + 64 * h + 16 * i + 4 * t);
+        for (int i = 0; i < 4; ++i) r[i] = ldw<AL>(at, b + 16 + 64 * h + 16 * i + 4 * t);
       } else if (FMT == LK_Q5_K) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = ldw<AL>(b + 48 + 64 * h + 16 * i + 4 * t);
+        for (int i = 0; i < 4; ++i) r[i] = ldw<AL>(at, b + 48 + 64 * h + 16 * i + 4 * t);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) r[4 + i] = ldw<AL>(b + 16 + 16 * i + 4 * t) >> (4 * h);
+        for (int i = 0; i < 2; ++i) r[4 + i] = ldw<AL>(at, b + 16 + 16 * i + 4 * t) >> (4 * h);
       } else if (FMT == LK_Q6_K) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = ldw<AL>(b + 64 * h + 16 * i + 4 * t);
+        for (int i = 0; i < 4; ++i) r[i] = ldw<AL>(at, b + 64 * h + 16 * i + 4 * t);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) r[4 + i] = ldw<AL>(b + 128 + 32 * h + 16 * i + 4 * t);
+        for (int i = 0; i < 2; ++i) r[4 + i] = ldw<AL>(at, b + 128 + 32 * h + 16 * i + 4 * t);
       } else {   // IQ4_XS
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = ldw<AL>(b + 8 + 64 * h + 16 * i + 4 * t);
+        for (int i = 0; i < 4; ++i) r[i] = ldw<AL>(at, b + 8 + 64 * h + 16 * i + 4 * t);
       }
     }
   }
@@ -165,29 +209,30 @@ struct Slice {
 
   // scale s of group t, and its minimum (Q4_K, Q5_K) or its second 16 values' scale (Q6_K) in m: this lane's share of
   // what the four lanes of a row exchange
-  LK_DEV static void scales(uint32_t p, int ks, int t, float& s, float& m) {
+  template <class At>
+  LK_DEV static void scales(const At& at, int ks, int t, float& s, float& m) {
     m = 0.0f;
     if (kQk == 32) {
-      s = lds_f16(p + (4 * ks + t) * kBb) * kInv0;
+      s = lds_f16(at, (4 * ks + t) * kBb) * kInv0;
       return;
     }
-    const uint32_t b = p + (ks >> 1) * kBb;
+    const uint32_t b = (ks >> 1) * kBb;
     const int j = 4 * (ks & 1) + t;
     if (FMT == LK_Q4_K || FMT == LK_Q5_K) {
-      const uint32_t dd = ldw<AL>(b), s0 = ldw<AL>(b + 4), s1 = ldw<AL>(b + 8), s2 = ldw<AL>(b + 12);
+      const uint32_t dd = ldw<AL>(at, b), s0 = ldw<AL>(at, b + 4), s1 = ldw<AL>(at, b + 8), s2 = ldw<AL>(at, b + 12);
       uint32_t sc, mn;
       q4k_scale_min_w(s0, s1, s2, j, sc, mn);
       s = h2f(uint16_t(dd & 0xffffu)) * float(sc) * ((t & 1) ? kInv1 : kInv0);
       m = h2f(uint16_t(dd >> 16)) * float(mn);
     } else if (FMT == LK_Q6_K) {
-      const uint32_t two = lds16(b + 192 + 2 * j);
-      const float d = lds_f16(b + 208) * kInv0;
+      const uint32_t two = lds16(at(b + 192 + 2 * j));
+      const float d = lds_f16(at, b + 208) * kInv0;
       s = d * float(int8_t(two & 255u));
       m = d * float(int8_t(two >> 8));
     } else {   // IQ4_XS
-      const uint32_t sh = lds16(b + 2), sl = ldw<AL>(b + 4);
+      const uint32_t sh = lds16(at(b + 2)), sl = ldw<AL>(at, b + 4);
       const int ls = int(((sl >> (4 * j)) & 15u) | (((sh >> (2 * j)) & 3u) << 4));
-      s = lds_f16(b) * float(ls - 32);
+      s = lds_f16(at, b) * float(ls - 32);
     }
   }
 
@@ -242,19 +287,91 @@ LK_DEV void store_q8(uint8_t* y, int64_t total, int64_t at, float v, int lane) {
     reinterpret_cast<float2*>(y + total)[at / 32] = make_float2(__half2float(__float2half_rn(d)), float(sum));
 }
 
-template <int FMT, bool AL, bool PAIR, int NT>
-__global__ void __launch_bounds__(kThreads, 1) k_mvx(const MvxArgs p) {
-  constexpr int kS = stages_of(FMT, NT), kSlot = slot_bytes(FMT, NT), kWSlot = slot_of(stage_bytes(FMT));
-  constexpr int kCB = stage_bytes(FMT), kT = 8 * NT;
+// 4 groups of 16 rows x 8 NT tokens: the warp's sums grow by the groups' dots. xa / ma: the shared-memory addresses of
+// the codes' word t (and 16 bytes on: word 4 + t) and of the meta of group j for this thread's tokens.
+template <int FMT, bool AL, int NT, class At, class XAt, class MAt>
+LK_DEV void slice_dot(const At& r0, const At& r1, int ks, int gc, int lane, const XAt& xa, const MAt& ma,
+                      float (&acc)[NT][4]) {
+  constexpr bool kTwo = FMT == LK_Q6_K, kMin = FMT == LK_Q4_K || FMT == LK_Q5_K;
+  const int t = lane & 3;
+  Slice<FMT, AL> w0, w1;
+  w0.load(r0, ks, t);
+  w1.load(r1, ks, t);
+  float s0, z0, s1, z1;
+  Slice<FMT, AL>::scales(r0, ks, t, s0, z0);
+  Slice<FMT, AL>::scales(r1, ks, t, s1, z1);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (j >= gc) break;
+    const int from = (lane & 28) | j;
+    const float a0 = __shfl_sync(0xFFFFFFFFu, s0, from), a1 = __shfl_sync(0xFFFFFFFFu, s1, from);
+    float b0 = 0.0f, b1 = 0.0f;
+    if (kTwo || kMin) {
+      b0 = __shfl_sync(0xFFFFFFFFu, z0, from);
+      b1 = __shfl_sync(0xFFFFFFFFu, z1, from);
+    }
+    uint32_t lo0, hi0, lo1, hi1;
+    w0.codes(j, lo0, hi0);
+    w1.codes(j, lo1, hi1);
+#pragma unroll
+    for (int q = 0; q < NT; ++q) {
+      const uint32_t x0 = lds(xa(q, j, 0)), x1 = lds(xa(q, j, 1));
+      float d[2], xs[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const uint32_t m = ma(q, c, j);
+        d[c] = __uint_as_float(lds(m));
+        if (kMin) xs[c] = d[c] * __uint_as_float(lds(m + 4));
+      }
+      float f[4];
+      if (kTwo) {
+        float h[4];
+        mma_k16(lo0, lo1, x0, f);
+        mma_k16(hi0, hi1, x1, h);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          acc[q][c] = fmaf(fmaf(h[c], c < 2 ? b0 : b1, f[c] * (c < 2 ? a0 : a1)), d[c & 1], acc[q][c]);
+      } else {
+        mma_k32<Slice<FMT, AL>::kUnsigned>(lo0, lo1, hi0, hi1, x0, x1, f);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          acc[q][c] = fmaf(f[c] * d[c & 1], c < 2 ? a0 : a1, acc[q][c]);
+          if (kMin) acc[q][c] = fmaf(-(c < 2 ? b0 : b1), xs[c & 1], acc[q][c]);
+        }
+      }
+    }
+  }
+}
+
+LK_DEV bool poll(uint64_t* bar, uint32_t phase) {
+  for (uint32_t q = 0; q < kWaitPolls; ++q)
+    if (mbar_try_wait(bar, phase)) return true;
+  return false;
+}
+
+template <int FMT, int FORM, bool PAIR, int NT>
+__global__ void __launch_bounds__(kThreads, 1)
+    k_mvx(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap w2map,
+          const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap mmap, const MvxArgs p) {
+  constexpr int kV = stage_values(NT), kCB = stage_bytes(FMT, kV), kWB = w_bytes(FMT, FORM, kV);
+  constexpr int kXB = x_bytes(FORM, NT, kV), kWSlot = slot_of(kCB), kT = 8 * NT;
+  constexpr int kXSlot = slot_of(kV), kMetaSlot = slot_of(kV / 4);   // row form
+  constexpr int kBoxRows = PAIR ? kRows / 2 : kRows, kPitch = kBoxRows * 128;
   constexpr int kOut = PAIR ? kRows / 2 : kRows;   // outputs of a tile
-  extern __shared__ __align__(128) uint8_t smem[];
-  float* red = reinterpret_cast<float*>(smem + kS * kSlot);            // [slice][token][36]
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kS * kSlot + red_bytes(NT));
-  uint64_t* empty = full + kS;
+  constexpr int kSub = kV / 1024;                  // 128-value parts of a warp's slice
+  // blocks and strides of Q4_K, Q5_K and IQ4_XS are multiples of 4 bytes; the box form's rows start on 16
+  constexpr bool kAL = FORM != kRowForm && fmt_block_bytes(FMT) % 4 == 0;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int nst = (p.k + kV - 1) / kV, groups = p.k / 32, kS = p.stages;
+  const int slot = kWB + (p.resident ? 0 : kXB);
+  uint8_t* xres = smem + kS * slot;                                    // resident activations
+  float* red = reinterpret_cast<float*>(xres + (p.resident ? nst * kXB : 0));   // [slice][token][36]
+  uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(red) + red_bytes(NT));
+  uint64_t* empty = full + kMaxStages;
   float* first = reinterpret_cast<float*>(full) + 64;                  // [32 tokens][16]: a unit's first tile
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t0 = blockIdx.y * kT, ntok = min(kT, p.tokens - t0);
-  const int nst = (p.k + kStageV - 1) / kStageV, groups = p.k / 32;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kS; ++i) {
       mbar_init(&full[i], 2);   // the weights' bytes and the activations' are announced apart
@@ -264,9 +381,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_mvx(const MvxArgs p) {
   }
   __syncthreads();
   mx_launch();
-  // tile row r: gate or up weight and its row (rows past n read row 0's bytes and are never stored)
+  // row form: tile row r, gate or up weight (rows past n read row 0's bytes and are never stored)
   auto row_src = [&](int tile, int r, int st) {
-    const int n = PAIR ? tile * kOut + (r & 15) : tile * kOut + r;
+    const int n = tile * kOut + (PAIR ? r & 15 : r);
     const uint8_t* b = PAIR && r >= 16 ? p.w2 : p.w;
     return reinterpret_cast<uintptr_t>(b) + uintptr_t(int64_t(n < p.n ? n : 0) * p.rb + int64_t(st) * kCB);
   };
@@ -274,28 +391,38 @@ __global__ void __launch_bounds__(kThreads, 1) k_mvx(const MvxArgs p) {
 
   if (warp == 0) {
     // ------------------------------------------------------------------ producer
-    bool live = true, waited = false;
-    int s = 0;
+    bool live = true, waited = false, used = false;   // used: the ring has been round once
+    int s = 0, round = 0;                              // round: tiles so far
     uint32_t turn = 0;
-    bool used = false;   // the ring has been round once
+    if (lane == 0 && FORM != kRowForm) {
+      prefetch_tensormap(&wmap);
+      if (PAIR) prefetch_tensormap(&w2map);
+    }
     for (int u = blockIdx.x; u < p.units && live; u += gridDim.x) {
-      for (int i = 0; i < p.tiles_per_unit && live; ++i) {
+      for (int i = 0; i < p.tiles_per_unit && live; ++i, ++round) {
         const int tile = u * p.tiles_per_unit + i;
         if (tile >= ntile) break;
         for (int st = 0; st < nst; ++st) {
-          if (used && !__all_sync(0xFFFFFFFFu, [&] {
-                for (uint32_t q = 0; q < kWaitPolls; ++q)
-                  if (mbar_try_wait(&empty[s], turn ^ 1)) return true;
-                return false;
-              }())) {
+          if (used && !__all_sync(0xFFFFFFFFu, poll(&empty[s], turn ^ 1))) {
             atomicOr(&g_status, 1u);
             live = false;
             break;
           }
-          uint8_t* dst = smem + s * kSlot;
-          {
+          uint8_t* dst = smem + s * slot;
+          const int64_t b0 = int64_t(st) * kCB;
+          const uint32_t len = uint32_t(min(int64_t(kCB), p.rb - b0));
+          if (FORM != kRowForm) {
+            if (lane == 0) {
+              const int seg0 = int(b0 >> 7), segs = int((b0 + len + 127) >> 7) - seg0;
+              mbar_expect_tx(&full[s], uint32_t(segs) * kRows * 128);
+              for (int g = 0; g < segs; ++g) {
+                tma_load_2d(dst + g * kPitch, &wmap, (seg0 + g) * 32, tile * kOut, &full[s]);
+                if (PAIR) tma_load_2d(dst + kWB / 2 + g * kPitch, &w2map, (seg0 + g) * 32, tile * kOut, &full[s]);
+              }
+            }
+          } else {
             const uintptr_t src = row_src(tile, lane, st);
-            const uint32_t len = uint32_t(min(int64_t(kCB), p.rb - int64_t(st) * kCB)), bytes = window(src, len);
+            const uint32_t bytes = window(src, len);
             uint32_t total = bytes;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
@@ -307,9 +434,27 @@ __global__ void __launch_bounds__(kThreads, 1) k_mvx(const MvxArgs p) {
             mx_wait();
             waited = true;
           }
-          {
-            const int gc = min(kStageV / 32, groups - st * (kStageV / 32));
-            const int64_t g0 = int64_t(t0 + lane) * groups + st * (kStageV / 32);
+          const int gc = min(kV / 32, groups - st * (kV / 32));   // groups of the stage
+          uint8_t* xd = p.resident ? xres + st * kXB : dst + kWB;
+          if (p.resident && round > 0) {
+            if (lane == 0) mbar_arrive(&full[s]);
+          } else if (FORM == kBox1) {
+            if (lane == 0) {
+              const int64_t g0 = int64_t(t0) * groups + st * (kV / 32);
+              mbar_expect_tx(&full[s], gc * 40);
+              bulk_g2s(xd, p.codes + g0 * 32, gc * 32, &full[s]);
+              bulk_g2s(xd + kV, p.meta + g0 * 8, gc * 8, &full[s]);
+            }
+          } else if (FORM == kBox) {
+            if (lane == 0) {
+              const int nc = (gc + 3) / 4, nm = (gc + 15) / 16;   // boxes of 128 codes, of 16 groups' meta
+              mbar_expect_tx(&full[s], uint32_t(nc + nm) * kT * 128);
+              for (int g = 0; g < nc; ++g) tma_load_2d(xd + g * kT * 128, &xmap, st * kV + g * 128, t0, &full[s]);
+              for (int g = 0; g < nm; ++g)
+                tma_load_2d(xd + kT * kV + g * kT * 128, &mmap, st * (kV / 16) + g * 32, t0, &full[s]);
+            }
+          } else {
+            const int64_t g0 = int64_t(t0 + lane) * groups + st * (kV / 32);
             const uintptr_t cs = reinterpret_cast<uintptr_t>(p.codes) + g0 * 32, ms = reinterpret_cast<uintptr_t>(p.meta) + g0 * 8;
             const uint32_t mb = window(ms, gc * 8);
             uint32_t total = lane < ntok ? gc * 32 + mb : 0;
@@ -318,11 +463,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_mvx(const MvxArgs p) {
             if (lane == 0) mbar_expect_tx(&full[s], total);
             __syncwarp();
             if (lane < ntok) {
-              uint8_t* xd = dst + kRows * kWSlot;
               bulk_g2s(xd + lane * kXSlot, reinterpret_cast<const void*>(cs), gc * 32, &full[s]);
               bulk_g2s(xd + kT * kXSlot + lane * kMetaSlot, reinterpret_cast<const void*>(ms & ~uintptr_t(15)), mb, &full[s]);
             }
           }
+          __syncwarp();
           if (++s == kS) {
             s = 0;
             turn ^= 1;
@@ -339,7 +484,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_mvx(const MvxArgs p) {
   // ------------------------------------------------------------------ consumers
   mx_wait();
   const int cw = warp - 1, half = cw >> 3, ks = cw & 7, g = lane >> 2, t = lane & 3;
-  const uint32_t sbase = smem_u32(smem);
+  const uint32_t sbase = smem_u32(smem), xbase = smem_u32(xres);
+  // this thread's activations inside a stage: codes of token 8 q + g, meta of tokens 8 q + 2 t and 8 q + 2 t + 1. Columns
+  // past the call's tokens repeat the last one (row form) or hold zeros (boxes), and are never stored.
+  uint32_t xoff[NT], moff[NT][2];
+#pragma unroll
+  for (int q = 0; q < NT; ++q) {
+    const int tok = 8 * q + g;
+    xoff[q] = FORM == kBox1 ? 4 * t : FORM == kBox ? tok * 128 + 4 * t : min(tok, ntok - 1) * kXSlot + 4 * t;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int tk = 8 * q + 2 * t + c, tr = min(tk, ntok - 1);
+      const uint32_t a = uint32_t(reinterpret_cast<uintptr_t>(p.meta)) + uint32_t(t0 + tr) * uint32_t(groups) * 8u;
+      moff[q][c] = FORM == kBox1 ? kV : FORM == kBox ? kT * kV + tk * 128 : kT * kXSlot + tr * kMetaSlot + (a & 15u);
+    }
+  }
   int s = 0;
   uint32_t turn = 0;
   bool live = true;
@@ -352,79 +511,42 @@ __global__ void __launch_bounds__(kThreads, 1) k_mvx(const MvxArgs p) {
       for (int q = 0; q < NT; ++q)
 #pragma unroll
         for (int c = 0; c < 4; ++c) acc[q][c] = 0.0f;
-      // low address bits of the two rows' windows: (row start + stage offset) mod 16
-      const uint32_t r0 = uint32_t(row_src(tile, 16 * half + g, 0)), r1 = uint32_t(row_src(tile, 16 * half + g + 8, 0));
-      const uint32_t m0 = uint32_t(reinterpret_cast<uintptr_t>(p.meta)) + uint32_t(t0) * uint32_t(groups) * 8u;
+      // row form: low address bits of the two rows' windows
+      const uint32_t a0 = uint32_t(row_src(tile, 16 * half + g, 0)), a1 = uint32_t(row_src(tile, 16 * half + g + 8, 0));
       for (int st = 0; st < nst; ++st) {
-        bool ok = false;
-        for (uint32_t q = 0; q < kWaitPolls && !ok; ++q) ok = mbar_try_wait(&full[s], turn);
-        if (!__all_sync(0xFFFFFFFFu, ok)) {
+        if (!__all_sync(0xFFFFFFFFu, poll(&full[s], turn))) {
           atomicOr(&g_status, 1u);
           live = false;
           break;
         }
-        const int gc = min(kStageV / 32, groups - st * (kStageV / 32)) - 4 * ks;   // groups of this slice
-        if (gc > 0) {
-          const uint32_t sb = sbase + s * kSlot;
-          const uint32_t p0 = sb + (16 * half + g) * kWSlot + ((r0 + uint32_t(st) * kCB) & 15u);
-          const uint32_t p1 = sb + (16 * half + g + 8) * kWSlot + ((r1 + uint32_t(st) * kCB) & 15u);
-          const uint32_t xb = sb + kRows * kWSlot + ks * 128 + 4 * t;                 // + token * kXSlot
-          const uint32_t mb = sb + kRows * kWSlot + kT * kXSlot + ks * 32;            // + token * kMetaSlot + window
-          Slice<FMT, AL> w0, w1;
-          w0.load(p0, ks, t);
-          w1.load(p1, ks, t);
-          float s0, z0, s1, z1;
-          Slice<FMT, AL>::scales(p0, ks, t, s0, z0);
-          Slice<FMT, AL>::scales(p1, ks, t, s1, z1);
+        const uint32_t sb = sbase + s * slot, xb = p.resident ? xbase + st * kXB : sb + kWB;
+        const int gst = min(kV / 32, groups - st * (kV / 32));
 #pragma unroll
-          for (int j = 0; j < kSliceG; ++j) {
-            if (j >= gc) break;
-            const int from = (lane & 28) | j;
-            const float a0 = __shfl_sync(0xFFFFFFFFu, s0, from), a1 = __shfl_sync(0xFFFFFFFFu, s1, from);
-            float b0 = 0.0f, b1 = 0.0f;
-            constexpr bool kTwo = FMT == LK_Q6_K, kMin = FMT == LK_Q4_K || FMT == LK_Q5_K;
-            if (kTwo || kMin) {
-              b0 = __shfl_sync(0xFFFFFFFFu, z0, from);
-              b1 = __shfl_sync(0xFFFFFFFFu, z1, from);
+        for (int sub = 0; sub < kSub; ++sub) {
+          const int part = ks * kSub + sub, gc = gst - 4 * part;   // which 128 values; groups left there
+          if (gc <= 0) break;
+          // codes and meta of group 4 part + j
+          auto xa = [&](int q, int j, int hi) {
+            if (FORM == kBox)   // one box per 128 values; chunk 2 j + hi of token row (8 q + g), g = row & 7
+              return xb + part * kT * 128 + (xoff[q] ^ uint32_t(((2 * j + hi) ^ g) << 4));
+            return xb + xoff[q] + part * 128 + 32 * j + 16 * hi;
+          };
+          auto ma = [&](int q, int c, int j) {
+            if (FORM == kBox) {   // one box per 16 groups: 16-byte chunk (group / 2) of token row
+              const int gg = 4 * (part & 3) + j;
+              return xb + (part >> 2) * kT * 128 + moff[q][c] + uint32_t(((gg >> 1) ^ (2 * t + c)) << 4) + 8 * (gg & 1);
             }
-            uint32_t lo0, hi0, lo1, hi1;
-            w0.codes(j, lo0, hi0);
-            w1.codes(j, lo1, hi1);
-#pragma unroll
-            for (int q = 0; q < NT; ++q) {
-              const int tok = 8 * q + g;
-              uint32_t x0 = 0, x1 = 0;
-              if (tok < ntok) {
-                x0 = lds(xb + tok * kXSlot + 32 * j);
-                x1 = lds(xb + tok * kXSlot + 32 * j + 16);
-              }
-              float d[2] = {0.0f, 0.0f}, xs[2] = {0.0f, 0.0f};
-#pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                const int tk = 8 * q + 2 * t + c;
-                if (tk < ntok) {
-                  const uint32_t a = mb + tk * kMetaSlot + ((m0 + uint32_t(tk) * uint32_t(groups) * 8u) & 15u) + 8 * j;
-                  d[c] = __uint_as_float(lds(a));
-                  if (kMin) xs[c] = d[c] * __uint_as_float(lds(a + 4));
-                }
-              }
-              float f[4];
-              if (kTwo) {
-                float h[4];
-                mma_k16(lo0, lo1, x0, f);
-                mma_k16(hi0, hi1, x1, h);
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                  acc[q][c] = fmaf(fmaf(h[c], c < 2 ? b0 : b1, f[c] * (c < 2 ? a0 : a1)), d[c & 1], acc[q][c]);
-              } else {
-                mma_k32<Slice<FMT, AL>::kUnsigned>(lo0, lo1, hi0, hi1, x0, x1, f);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                  acc[q][c] = fmaf(f[c] * d[c & 1], c < 2 ? a0 : a1, acc[q][c]);
-                  if (kMin) acc[q][c] = fmaf(-(c < 2 ? b0 : b1), xs[c & 1], acc[q][c]);
-                }
-              }
-            }
+            return xb + moff[q][c] + part * 32 + 8 * j;
+          };
+          if (FORM == kRowForm) {
+            const RowAt r0{sb + (16 * half + g) * kWSlot + ((a0 + uint32_t(st) * kCB) & 15u)};
+            const RowAt r1{sb + (16 * half + g + 8) * kWSlot + ((a1 + uint32_t(st) * kCB) & 15u)};
+            slice_dot<FMT, kAL, NT>(r0, r1, part, gc, lane, xa, ma, acc);
+          } else {
+            const uint32_t off = uint32_t(int64_t(st) * kCB) & 127u;
+            const uint32_t base = sb + (PAIR ? half * (kWB / 2) : half * 16 * 128) + g * 128;
+            const BoxAt<kPitch> r0{base, off, uint32_t(g) << 4}, r1{base + 8 * 128, off, uint32_t(g) << 4};
+            slice_dot<FMT, kAL, NT>(r0, r1, part, gc, lane, xa, ma, acc);
           }
         }
         __syncwarp();
@@ -485,15 +607,25 @@ __global__ void __launch_bounds__(kThreads, 1) k_mvx(const MvxArgs p) {
   }
 }
 
-template <int FMT, bool AL, bool PAIR, int NT>
-int launch(const MvxArgs& a, cudaStream_t s) {
-  constexpr int kS = stages_of(FMT, NT);
-  static_assert(kS >= 2, "two stages at least");
-  static_assert(kS * 16 <= 256 && kTailBytes >= 256 + 32 * 16 * 4, "the tail");
-  constexpr int smem = kS * slot_bytes(FMT, NT) + red_bytes(NT) + kTailBytes;
-  auto kern = k_mvx<FMT, AL, PAIR, NT>;
+struct Maps {
+  CUtensorMap w, w2, x, m;
+};
+
+template <int FMT, int FORM, bool PAIR, int NT>
+int launch(const Maps& m, MvxArgs a, cudaStream_t s) {
+  constexpr int kV = stage_values(NT), kWB = w_bytes(FMT, FORM, kV), kXB = x_bytes(FORM, NT, kV);
+  constexpr int kFixed = 1024 + red_bytes(NT) + kTailBytes;
+  static_assert(2 * (kWB + kXB) + kFixed <= kSmemMax, "two stages at least");
+  static_assert(2 * kMaxStages * 8 <= 256, "the barriers");
+  const int nst = (a.k + kV - 1) / kV;
+  // the activations stay where they leave three stages of weights (two for the widest rows of 8 tokens and fewer)
+  a.resident = FORM != kRowForm && int64_t(nst) * kXB + (NT == 1 ? 2 : 3) * kWB + kFixed <= kSmemMax;
+  const int room = kSmemMax - kFixed - (a.resident ? nst * kXB : 0), slot = kWB + (a.resident ? 0 : kXB);
+  a.stages = room / slot < kMaxStages ? room / slot : kMaxStages;
+  const int smem = kFixed + a.stages * slot + (a.resident ? nst * kXB : 0);
+  auto kern = k_mvx<FMT, FORM, PAIR, NT>;
   static unsigned configured = 0;
-  if (!once_per_device(configured)) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (!once_per_device(configured)) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
   int dev = 0, sms = 0;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
@@ -507,19 +639,39 @@ int launch(const MvxArgs& a, cudaStream_t s) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, a) == cudaSuccess ? LK_OK : LK_ECUDA;
+  return cudaLaunchKernelEx(&cfg, kern, m.w, m.w2, m.x, m.m, a) == cudaSuccess ? LK_OK : LK_ECUDA;
 }
 
-template <int FMT, bool AL>
+template <int FMT, int FORM, bool PAIR>
+int launch_t(const Maps& m, const MvxArgs& a, cudaStream_t s) {
+  if (FORM == kBox1 || a.tokens <= 8) return launch<FMT, FORM, PAIR, 1>(m, a, s);
+  if (a.tokens <= 16) return launch<FMT, FORM == kBox1 ? kBox : FORM, PAIR, 2>(m, a, s);
+  return launch<FMT, FORM == kBox1 ? kBox : FORM, PAIR, 4>(m, a, s);
+}
+
+template <int FMT>
 int launch_f(const MvxArgs& a, cudaStream_t s) {
-  if (a.w2) {
-    if (a.tokens <= 8) return launch<FMT, AL, true, 1>(a, s);
-    if (a.tokens <= 16) return launch<FMT, AL, true, 2>(a, s);
-    return launch<FMT, AL, true, 4>(a, s);
+  auto al16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  const bool pair = a.w2 != nullptr;
+  // boxes: rows, codes and meta at 16-byte strides from 16-byte aligned starts
+  const bool box = a.rb % 16 == 0 && al16(a.w) && al16(a.w2) && a.k % 64 == 0 && a.k >= 256;
+  Maps m;
+  if (!box) {
+    memset(&m, 0, sizeof(m));
+    return pair ? launch_t<FMT, kRowForm, true>(m, a, s) : launch_t<FMT, kRowForm, false>(m, a, s);
   }
-  if (a.tokens <= 8) return launch<FMT, AL, false, 1>(a, s);
-  if (a.tokens <= 16) return launch<FMT, AL, false, 2>(a, s);
-  return launch<FMT, AL, false, 4>(a, s);
+  const int rows = pair ? kRows / 2 : kRows, kt = a.tokens <= 8 ? 8 : a.tokens <= 16 ? 16 : 32;
+  int rc = make_map(&m.w, a.w, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, a.n, a.rb / 4, 32, rows, CU_TENSOR_MAP_SWIZZLE_128B);
+  m.w2 = m.x = m.m = m.w;
+  if (rc == LK_OK && pair)
+    rc = make_map(&m.w2, a.w2, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, a.n, a.rb / 4, 32, rows, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc == LK_OK && a.tokens > 1)
+    rc = make_map(&m.x, a.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.tokens, a.k, 128, kt, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc == LK_OK && a.tokens > 1)
+    rc = make_map(&m.m, a.meta, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, a.tokens, a.k / 16, 32, kt, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc != LK_OK) return rc;
+  if (a.tokens == 1) return pair ? launch_t<FMT, kBox1, true>(m, a, s) : launch_t<FMT, kBox1, false>(m, a, s);
+  return pair ? launch_t<FMT, kBox, true>(m, a, s) : launch_t<FMT, kBox, false>(m, a, s);
 }
 
 }  // namespace
@@ -540,17 +692,15 @@ int mv_q8_ex(int fmt, int n, int k, int tokens, const uint8_t* xq, const void* w
   a.tiles_per_unit = w2 && e.y_form == LK_Q8_ROWS ? 2 : 1;
   a.units = (tiles + a.tiles_per_unit - 1) / a.tiles_per_unit;
   if (int64_t(tokens) > 65535 * 32) return LK_ERANGE;
-  // whole words where blocks and rows are multiples of 4 bytes (Q4_K, Q5_K, IQ4_XS) from a 4-byte aligned start
-  const bool al = ((reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(w2)) & 3) == 0;
   switch (fmt) {
-    case LK_Q4_0: return launch_f<LK_Q4_0, false>(a, s);
-    case LK_Q8_0: return launch_f<LK_Q8_0, false>(a, s);
-    case LK_Q5_0: return launch_f<LK_Q5_0, false>(a, s);
-    case LK_Q6_K: return launch_f<LK_Q6_K, false>(a, s);
-    case LK_IQ4_NL: return launch_f<LK_IQ4_NL, false>(a, s);
-    case LK_Q4_K: return al ? launch_f<LK_Q4_K, true>(a, s) : launch_f<LK_Q4_K, false>(a, s);
-    case LK_Q5_K: return al ? launch_f<LK_Q5_K, true>(a, s) : launch_f<LK_Q5_K, false>(a, s);
-    case LK_IQ4_XS: return al ? launch_f<LK_IQ4_XS, true>(a, s) : launch_f<LK_IQ4_XS, false>(a, s);
+    case LK_Q4_0: return launch_f<LK_Q4_0>(a, s);
+    case LK_Q4_K: return launch_f<LK_Q4_K>(a, s);
+    case LK_Q8_0: return launch_f<LK_Q8_0>(a, s);
+    case LK_Q5_0: return launch_f<LK_Q5_0>(a, s);
+    case LK_Q5_K: return launch_f<LK_Q5_K>(a, s);
+    case LK_Q6_K: return launch_f<LK_Q6_K>(a, s);
+    case LK_IQ4_NL: return launch_f<LK_IQ4_NL>(a, s);
+    case LK_IQ4_XS: return launch_f<LK_IQ4_XS>(a, s);
   }
   return LK_EUNSUPPORTED;
 }
