@@ -93,146 +93,232 @@ LK_DEV uint32_t lds16(uint32_t a) {
   asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
   return v;
 }
-// Where byte b of a weight row's stage sits in shared memory. Row form: linear from the row's window.
+LK_DEV uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+// four 8 x 16-byte matrices: lane l supplies the address of row l % 8 of matrix l / 8, and gets word l % 4 of row l / 4 of
+// each -- the operand layout of the MMAs
+LK_DEV void ldmatrix4(uint32_t a, uint32_t& m0, uint32_t& m1, uint32_t& m2, uint32_t& m3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(m0), "=r"(m1), "=r"(m2), "=r"(m3)
+               : "r"(a));
+}
+
+// Where byte b of a stage of this thread's two tile rows (g and g + 8) sits in shared memory, and loads of both.
+// Row form: linear from each row's window, at any 2-byte alignment.
 struct RowAt {
-  uint32_t p;
-  LK_DEV uint32_t operator()(uint32_t b) const { return p + b; }
+  static constexpr bool kBoxes = false;
+  uint32_t p[2];
+  LK_DEV static uint32_t one(uint32_t a) {
+    const uint32_t c = a & ~3u;
+    return __funnelshift_r(lds(c), lds(c + 4), (a & 3u) * 8u);
+  }
+  template <int LOW>
+  LK_DEV void word(uint32_t b, uint32_t& u, uint32_t& v) const {
+    u = one(p[0] + b);
+    v = one(p[1] + b);
+  }
+  LK_DEV void half(uint32_t b, uint32_t& u, uint32_t& v) const {
+    u = lds16(p[0] + b);
+    v = lds16(p[1] + b);
+  }
 };
-// Box form: 128-byte segments, `pitch` bytes apart, of swizzled rows (16-byte chunk c of row r at c ^ (r & 7))
+// Box form: 128-byte segments, PITCH bytes apart, of swizzled rows (16-byte chunk c of row r at c ^ (r & 7)); row g + 8
+// is 1024 bytes on with the same swizzle
 template <int PITCH>
 struct BoxAt {
-  uint32_t p, off, x;   // the row in segment 0; the stage's first byte in it; (row & 7) << 4
-  LK_DEV uint32_t operator()(uint32_t b) const {
+  static constexpr bool kBoxes = true;
+  uint32_t p, off, x;      // row g in segment 0; the stage's first byte in it; (g & 7) << 4
+  uint32_t mp, mx, mb;     // the row, its swizzle and the 16-byte step this lane supplies to ldmatrix4
+  LK_DEV uint32_t at(uint32_t b) const {
     b += off;
     return p + (b >> 7) * PITCH + ((b & 0x7Fu) ^ x);
   }
+  // rows g and g + 8 of the 16-byte chunks at b (words t in u0, v0) and b + 16 (u1, v1)
+  LK_DEV void chunks(uint32_t b, uint32_t& u0, uint32_t& v0, uint32_t& u1, uint32_t& v1) const {
+    b += off + mb;
+    ldmatrix4(mp + (b >> 7) * PITCH + ((b & 0x7Fu) ^ mx), u0, v0, u1, v1);
+  }
+  // LOW: b mod 4 where it is known, else -1 (even)
+  template <int LOW>
+  LK_DEV void word(uint32_t b, uint32_t& u, uint32_t& v) const {
+    if (LOW == 0) {
+      const uint32_t a = at(b);
+      u = lds(a);
+      v = lds(a + 1024);
+      return;
+    }
+    const uint32_t lo = at(b & ~3u), hi = at((b & ~3u) + 4), sh = LOW == 2 ? 16u : (b & 3u) * 8u;
+    u = __funnelshift_r(lds(lo), lds(hi), sh);
+    v = __funnelshift_r(lds(lo + 1024), lds(hi + 1024), sh);
+  }
+  LK_DEV void half(uint32_t b, uint32_t& u, uint32_t& v) const {
+    const uint32_t a = at(b);
+    u = lds16(a);
+    v = lds16(a + 1024);
+  }
 };
-// the word at byte b, 2-byte aligned (AL: known to be 4-byte aligned)
-template <bool AL, class At>
-LK_DEV uint32_t ldw(const At& at, uint32_t b) {
-  if (AL) return lds(at(b));
-  const uint32_t lo = at(b & ~3u), hi = at((b & ~3u) + 4);
-  // the row form's start may itself be off a word: its at() keeps the low bits
-  return __funnelshift_r(lds(lo), lds(hi), (b & 3u) * 8u);
-}
-template <bool AL>
-LK_DEV uint32_t ldw(const RowAt& at, uint32_t b) {
-  const uint32_t a = at(b);
-  if (AL) return lds(a);
-  const uint32_t c = a & ~3u;
-  return __funnelshift_r(lds(c), lds(c + 4), (a & 3u) * 8u);
-}
-template <class At>
-LK_DEV float lds_f16(const At& at, uint32_t b) { return h2f(uint16_t(lds16(at(b)))); }
 
-// One weight row's slice of 4 groups: the packed words a thread (t = lane & 3) contributes to the MMAs. For group j,
-// lo(j) holds the codes of values 4t .. 4t + 3 and hi(j) those of 16 + 4t .. 16 + 4t + 3, one per byte, as UNSIGNED ? u8 :
-// s8 times 2^SHIFT.
-template <int FMT, bool AL>
+// 128 values (4 groups) of a thread's two tile rows: the packed words it contributes to the MMAs (t = lane & 3). For
+// group j and row i, lo holds the codes of values 4t .. 4t + 3 and hi those of 16 + 4t .. 16 + 4t + 3, one per byte, u8 or
+// s8, times the power of two that its scale divides by.
+template <int FMT>
 struct Slice {
   static constexpr bool kUnsigned = FMT == LK_Q4_K || FMT == LK_Q5_K;
   static constexpr int kQk = fmt_qk(FMT), kBb = fmt_block_bytes(FMT);
-  uint32_t r[FMT == LK_Q8_0 || FMT == LK_Q5_0 ? 8 : FMT == LK_Q5_K || FMT == LK_Q6_K ? 6 : 4];
+  // b mod 4 of a field at byte c of block j: known for blocks of an even number of 4-byte words, or where j is
+  static constexpr int low(int c, int j) { return (j * kBb + c) % 4; }
+  uint32_t r[2][FMT == LK_Q8_0 || FMT == LK_Q5_0 ? 8 : FMT == LK_Q5_K || FMT == LK_Q6_K ? 6 : 4];
 
-  // at: the row's stage in shared memory; ks: which 128 values of it
-  template <class At>
-  LK_DEV void load(const At& at, int ks, int t) {
-    if (kQk == 32) {
+  template <int J, class At>
+  LK_DEV void load_block(const At& at, uint32_t b, int t) {
+    if (FMT == LK_Q8_0) {
+      at.template word<low(2, J)>(b + 2 + 4 * t, r[0][2 * J], r[1][2 * J]);
+      at.template word<low(2, J)>(b + 18 + 4 * t, r[0][2 * J + 1], r[1][2 * J + 1]);
+    } else if (FMT == LK_Q5_0) {
+      at.template word<low(6, J)>(b + 6 + 4 * t, r[0][2 * J], r[1][2 * J]);
+      // bits 4t .. 4t + 3 and 16 + 4t .. of qh, in one word: bits 0-3 and 16-19
+      at.template word<low(2, J)>(b + 2, r[0][2 * J + 1], r[1][2 * J + 1]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t b = (4 * ks + j) * kBb;
-        if (FMT == LK_Q8_0) {
-          r[2 * j] = ldw<AL>(at, b + 2 + 4 * t);
-          r[2 * j + 1] = ldw<AL>(at, b + 18 + 4 * t);
-        } else if (FMT == LK_Q5_0) {
-          r[2 * j] = ldw<AL>(at, b + 6 + 4 * t);
-          // bits 4t .. 4t + 3 and 16 + 4t .. of qh, in one word: bits 0-3 and 16-19
-          r[2 * j + 1] = (ldw<AL>(at, b + 2) >> (4 * t)) & 0x000F000Fu;
-        } else {
-          r[j] = ldw<AL>(at, b + 2 + 4 * t);
-        }
-      }
+      for (int i = 0; i < 2; ++i) r[i][2 * J + 1] = (r[i][2 * J + 1] >> (4 * t)) & 0x000F000Fu;
     } else {
-      const uint32_t b = (ks >> 1) * kBb;   // the slice is half a super-block: groups 4 h .. 4 h + 3
-      const int h = ks & 1;
-      if (FMT == LK_Q4_K) {
+      at.template word<low(2, J)>(b + 2 + 4 * t, r[0][J], r[1][J]);
+    }
+  }
+  // part: which 128 values of the stage
+  template <class At>
+  LK_DEV void load(const At& at, int part, int t) {
+    if constexpr (kQk == 32) {
+      const uint32_t b = 4 * part * kBb;   // a multiple of 8
+      load_block<0>(at, b, t);
+      load_block<1>(at, b + kBb, t);
+      load_block<2>(at, b + 2 * kBb, t);
+      load_block<3>(at, b + 3 * kBb, t);
+    } else {
+      const uint32_t b = (part >> 1) * kBb;   // half a super-block: groups 4 h .. 4 h + 3
+      const int h = part & 1;
+      if constexpr ((FMT == LK_Q4_K || FMT == LK_Q5_K) && At::kBoxes) {
+        constexpr int kQs = FMT == LK_Q4_K ? 16 : 48;
+        at.chunks(b + kQs + 64 * h, r[0][0], r[1][0], r[0][1], r[1][1]);
+        at.chunks(b + kQs + 64 * h + 32, r[0][2], r[1][2], r[0][3], r[1][3]);
+        if constexpr (FMT == LK_Q5_K) {
+          at.chunks(b + 16, r[0][4], r[1][4], r[0][5], r[1][5]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = ldw<AL>(at, b + 16 + 64 * h + 16 * i + 4 * t);
-      } else if (FMT == LK_Q5_K) {
+          for (int i = 0; i < 2; ++i) {
+            r[i][4] >>= 4 * h;
+            r[i][5] >>= 4 * h;
+          }
+        }
+      } else if constexpr (FMT == LK_Q4_K || FMT == LK_Q5_K || FMT == LK_IQ4_XS) {
+        constexpr int kQs = FMT == LK_Q4_K ? 16 : FMT == LK_Q5_K ? 48 : 8;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = ldw<AL>(at, b + 48 + 64 * h + 16 * i + 4 * t);
+        for (int i = 0; i < 4; ++i) at.template word<0>(b + kQs + 64 * h + 16 * i + 4 * t, r[0][i], r[1][i]);
+        if constexpr (FMT == LK_Q5_K) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) r[4 + i] = ldw<AL>(at, b + 16 + 16 * i + 4 * t) >> (4 * h);
-      } else if (FMT == LK_Q6_K) {
+          for (int i = 0; i < 2; ++i) {
+            at.template word<0>(b + 16 + 16 * i + 4 * t, r[0][4 + i], r[1][4 + i]);
+            r[0][4 + i] >>= 4 * h;
+            r[1][4 + i] >>= 4 * h;
+          }
+        }
+      } else {   // Q6_K
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = ldw<AL>(at, b + 64 * h + 16 * i + 4 * t);
+        for (int i = 0; i < 4; ++i) at.template word<-1>(b + 64 * h + 16 * i + 4 * t, r[0][i], r[1][i]);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) r[4 + i] = ldw<AL>(at, b + 128 + 32 * h + 16 * i + 4 * t);
-      } else {   // IQ4_XS
-#pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = ldw<AL>(at, b + 8 + 64 * h + 16 * i + 4 * t);
+        for (int i = 0; i < 2; ++i)
+          at.template word<-1>(b + 128 + 32 * h + 16 * i + 4 * t, r[0][4 + i], r[1][4 + i]);
       }
     }
   }
 
-  // the codes of group j (0..3)
-  LK_DEV void codes(int j, uint32_t& lo, uint32_t& hi) const {
+  // the codes of group j (0..3) of row i
+  LK_DEV void codes(int i, int j, uint32_t& lo, uint32_t& hi) const {
     constexpr uint32_t kLow = 0x0F0F0F0Fu, kHigh = 0xF0F0F0F0u, kTop = 0x80808080u;
-    if (FMT == LK_Q4_0) {            // 16 (q - 8)
-      lo = ((r[j] << 4) & kHigh) ^ kTop;
-      hi = (r[j] & kHigh) ^ kTop;
-    } else if (FMT == LK_IQ4_NL || FMT == LK_IQ4_XS) {
-      lo = iq4_lookup4(r[j] & kLow) ^ kTop;
-      hi = iq4_lookup4((r[j] >> 4) & kLow) ^ kTop;
-    } else if (FMT == LK_Q8_0) {
-      lo = r[2 * j];
-      hi = r[2 * j + 1];
-    } else if (FMT == LK_Q5_0) {     // 8 (q - 16): the nibble at bit 3, the fifth bit at 7
-      const uint32_t q = r[2 * j], b = r[2 * j + 1];
+    const uint32_t* w = r[i];
+    if constexpr (FMT == LK_Q4_0) {            // 16 (q - 8)
+      lo = ((w[j] << 4) & kHigh) ^ kTop;
+      hi = (w[j] & kHigh) ^ kTop;
+    } else if constexpr (FMT == LK_IQ4_NL || FMT == LK_IQ4_XS) {
+      lo = iq4_lookup4(w[j] & kLow) ^ kTop;
+      hi = iq4_lookup4((w[j] >> 4) & kLow) ^ kTop;
+    } else if constexpr (FMT == LK_Q8_0) {
+      lo = w[2 * j];
+      hi = w[2 * j + 1];
+    } else if constexpr (FMT == LK_Q5_0) {     // 8 (q - 16): the nibble at bit 3, the fifth bit at 7
+      const uint32_t q = w[2 * j], b = w[2 * j + 1];
       lo = (((q & kLow) << 3) | spread(b)) ^ kTop;
       hi = (((q >> 1) & 0x78787878u) | spread(b >> 16)) ^ kTop;
-    } else if (FMT == LK_Q4_K) {     // page j / 2: even groups q, odd groups 16 q
+    } else if constexpr (FMT == LK_Q4_K) {     // page j / 2: even groups q, odd groups 16 q
       const uint32_t m = (j & 1) ? kHigh : kLow;
-      lo = r[2 * (j >> 1)] & m;
-      hi = r[2 * (j >> 1) + 1] & m;
-    } else if (FMT == LK_Q5_K) {     // nibble | bit j << 4
-      lo = ((r[2 * (j >> 1)] >> (4 * (j & 1))) & kLow) | (((r[4] >> j) & 0x01010101u) << 4);
-      hi = ((r[2 * (j >> 1) + 1] >> (4 * (j & 1))) & kLow) | (((r[5] >> j) & 0x01010101u) << 4);
-    } else if (FMT == LK_Q6_K) {     // 4 (q - 32): nibble at bit 2, the two high bits at 6
-      lo = six(r[2 * (j & 1)], r[4], j);
-      hi = six(r[2 * (j & 1) + 1], r[5], j);
+      lo = w[2 * (j >> 1)] & m;
+      hi = w[2 * (j >> 1) + 1] & m;
+    } else if constexpr (FMT == LK_Q5_K) {     // nibble | bit j << 4
+      lo = ((w[2 * (j >> 1)] >> (4 * (j & 1))) & kLow) | (((w[4] >> j) & 0x01010101u) << 4);
+      hi = ((w[2 * (j >> 1) + 1] >> (4 * (j & 1))) & kLow) | (((w[5] >> j) & 0x01010101u) << 4);
+    } else {                                   // Q6_K: 4 (q - 32): nibble at bit 2, the two high bits at 6
+      lo = six(w[2 * (j & 1)], w[4], j);
+      hi = six(w[2 * (j & 1) + 1], w[5], j);
     }
   }
   // factor of the codes' scale
-  static constexpr float kInv0 = FMT == LK_Q4_0 ? 0.0625f : FMT == LK_Q5_0 ? 0.125f : FMT == LK_Q6_K ? 0.25f : 1.0f;
-  static constexpr float kInv1 = FMT == LK_Q4_K ? 0.0625f : kInv0;   // odd groups
+  [[maybe_unused]] static constexpr float kInv0 = FMT == LK_Q4_0 ? 0.0625f : FMT == LK_Q5_0 ? 0.125f : FMT == LK_Q6_K ? 0.25f : 1.0f;
+  [[maybe_unused]] static constexpr float kInv1 = FMT == LK_Q4_K ? 0.0625f : kInv0;   // odd groups
 
-  // scale s of group t, and its minimum (Q4_K, Q5_K) or its second 16 values' scale (Q6_K) in m: this lane's share of
-  // what the four lanes of a row exchange
+  // scales s of group t of both rows, and their minima (Q4_K, Q5_K) or second 16 values' scales (Q6_K) in m: this lane's
+  // share of what the four lanes of a row exchange
   template <class At>
-  LK_DEV static void scales(const At& at, int ks, int t, float& s, float& m) {
-    m = 0.0f;
-    if (kQk == 32) {
-      s = lds_f16(at, (4 * ks + t) * kBb) * kInv0;
+  LK_DEV static void scales(const At& at, int part, int t, float (&s)[2], float (&m)[2]) {
+    m[0] = m[1] = 0.0f;
+    uint32_t d[2];
+    if constexpr (kQk == 32) {
+      at.half((4 * part + t) * kBb, d[0], d[1]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) s[i] = h2f(uint16_t(d[i])) * kInv0;
       return;
     }
-    const uint32_t b = (ks >> 1) * kBb;
-    const int j = 4 * (ks & 1) + t;
-    if (FMT == LK_Q4_K || FMT == LK_Q5_K) {
-      const uint32_t dd = ldw<AL>(at, b), s0 = ldw<AL>(at, b + 4), s1 = ldw<AL>(at, b + 8), s2 = ldw<AL>(at, b + 12);
-      uint32_t sc, mn;
-      q4k_scale_min_w(s0, s1, s2, j, sc, mn);
-      s = h2f(uint16_t(dd & 0xffffu)) * float(sc) * ((t & 1) ? kInv1 : kInv0);
-      m = h2f(uint16_t(dd >> 16)) * float(mn);
-    } else if (FMT == LK_Q6_K) {
-      const uint32_t two = lds16(at(b + 192 + 2 * j));
-      const float d = lds_f16(at, b + 208) * kInv0;
-      s = d * float(int8_t(two & 255u));
-      m = d * float(int8_t(two >> 8));
+    const uint32_t b = (part >> 1) * kBb;
+    const int j = 4 * (part & 1) + t;
+    if constexpr (FMT == LK_Q4_K || FMT == LK_Q5_K) {
+      uint4 h[2];
+      if constexpr (At::kBoxes) {
+        const uint32_t a = at.at(b);
+        h[0] = lds128(a);
+        h[1] = lds128(a + 1024);
+      } else {
+        at.template word<0>(b, h[0].x, h[1].x);
+        at.template word<0>(b + 4, h[0].y, h[1].y);
+        at.template word<0>(b + 8, h[0].z, h[1].z);
+        at.template word<0>(b + 12, h[0].w, h[1].w);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint32_t sc, mn;
+        q4k_scale_min_w(h[i].y, h[i].z, h[i].w, j, sc, mn);
+        s[i] = h2f(uint16_t(h[i].x & 0xffffu)) * float(sc) * ((t & 1) ? kInv1 : kInv0);
+        m[i] = h2f(uint16_t(h[i].x >> 16)) * float(mn);
+      }
+    } else if constexpr (FMT == LK_Q6_K) {
+      uint32_t two[2];
+      at.half(b + 192 + 2 * j, two[0], two[1]);
+      at.half(b + 208, d[0], d[1]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float f = h2f(uint16_t(d[i])) * kInv0;
+        s[i] = f * float(int8_t(two[i] & 255u));
+        m[i] = f * float(int8_t(two[i] >> 8));
+      }
     } else {   // IQ4_XS
-      const uint32_t sh = lds16(at(b + 2)), sl = ldw<AL>(at, b + 4);
-      const int ls = int(((sl >> (4 * j)) & 15u) | (((sh >> (2 * j)) & 3u) << 4));
-      s = lds_f16(at, b) * float(ls - 32);
+      uint32_t sh[2], sl[2];
+      at.half(b, d[0], d[1]);
+      at.half(b + 2, sh[0], sh[1]);
+      at.template word<0>(b + 4, sl[0], sl[1]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int ls = int(((sl[i] >> (4 * j)) & 15u) | (((sh[i] >> (2 * j)) & 3u) << 4));
+        s[i] = h2f(uint16_t(d[i])) * float(ls - 32);
+      }
     }
   }
 
@@ -287,56 +373,62 @@ LK_DEV void store_q8(uint8_t* y, int64_t total, int64_t at, float v, int lane) {
     reinterpret_cast<float2*>(y + total)[at / 32] = make_float2(__half2float(__float2half_rn(d)), float(sum));
 }
 
-// 4 groups of 16 rows x 8 NT tokens: the warp's sums grow by the groups' dots. xa / ma: the shared-memory addresses of
-// the codes' word t (and 16 bytes on: word 4 + t) and of the meta of group j for this thread's tokens.
-template <int FMT, bool AL, int NT, class At, class XAt, class MAt>
-LK_DEV void slice_dot(const At& r0, const At& r1, int ks, int gc, int lane, const XAt& xa, const MAt& ma,
-                      float (&acc)[NT][4]) {
+// 4 groups of 16 rows x 8 NT tokens: the warp's sums grow by the groups' dots. x(q, pr, w): the codes' words of groups
+// 2 pr and 2 pr + 1 for token 8 q + g; m(q, c, pr): (scale, sum of codes) of those groups for token 8 q + 2 t + c. COLS: the
+// columns a thread keeps (1 where the call has one token).
+template <int FMT, int NT, int COLS, class At, class XAt, class MAt>
+LK_DEV void slice_dot(const At& at, int part, int gc, int lane, const XAt& x, const MAt& m, float (&acc)[NT][4]) {
   constexpr bool kTwo = FMT == LK_Q6_K, kMin = FMT == LK_Q4_K || FMT == LK_Q5_K;
   const int t = lane & 3;
-  Slice<FMT, AL> w0, w1;
-  w0.load(r0, ks, t);
-  w1.load(r1, ks, t);
-  float s0, z0, s1, z1;
-  Slice<FMT, AL>::scales(r0, ks, t, s0, z0);
-  Slice<FMT, AL>::scales(r1, ks, t, s1, z1);
+  Slice<FMT> w;
+  w.load(at, part, t);
+  float s[2], z[2];
+  Slice<FMT>::scales(at, part, t, s, z);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (j >= gc) break;
-    const int from = (lane & 28) | j;
-    const float a0 = __shfl_sync(0xFFFFFFFFu, s0, from), a1 = __shfl_sync(0xFFFFFFFFu, s1, from);
-    float b0 = 0.0f, b1 = 0.0f;
-    if (kTwo || kMin) {
-      b0 = __shfl_sync(0xFFFFFFFFu, z0, from);
-      b1 = __shfl_sync(0xFFFFFFFFu, z1, from);
+  for (int pr = 0; pr < 2; ++pr) {
+    if (2 * pr >= gc) break;
+    uint32_t lo[2][2], hi[2][2];   // [group][row]
+    float a[2][2], b[2][2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int j = 2 * pr + k, from = (lane & 28) | j;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        a[k][i] = __shfl_sync(0xFFFFFFFFu, s[i], from);
+        if (kTwo || kMin) b[k][i] = __shfl_sync(0xFFFFFFFFu, z[i], from);
+        w.codes(i, j, lo[k][i], hi[k][i]);
+      }
     }
-    uint32_t lo0, hi0, lo1, hi1;
-    w0.codes(j, lo0, hi0);
-    w1.codes(j, lo1, hi1);
 #pragma unroll
     for (int q = 0; q < NT; ++q) {
-      const uint32_t x0 = lds(xa(q, j, 0)), x1 = lds(xa(q, j, 1));
-      float d[2], xs[2];
+      uint32_t xw[4];
+      x(q, pr, xw);
+      uint4 mt[2];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const uint32_t m = ma(q, c, j);
-        d[c] = __uint_as_float(lds(m));
-        if (kMin) xs[c] = d[c] * __uint_as_float(lds(m + 4));
-      }
-      float f[4];
-      if (kTwo) {
-        float h[4];
-        mma_k16(lo0, lo1, x0, f);
-        mma_k16(hi0, hi1, x1, h);
+      for (int c = 0; c < COLS; ++c) mt[c] = m(q, c, pr);
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-          acc[q][c] = fmaf(fmaf(h[c], c < 2 ? b0 : b1, f[c] * (c < 2 ? a0 : a1)), d[c & 1], acc[q][c]);
-      } else {
-        mma_k32<Slice<FMT, AL>::kUnsigned>(lo0, lo1, hi0, hi1, x0, x1, f);
+      for (int k = 0; k < 2; ++k) {
+        if (!At::kBoxes && 2 * pr + k >= gc) break;   // box form: an even number of groups
+        float f[4], h[4];
+        if (kTwo) {
+          mma_k16(lo[k][0], lo[k][1], xw[2 * k], f);
+          mma_k16(hi[k][0], hi[k][1], xw[2 * k + 1], h);
+        } else {
+          mma_k32<Slice<FMT>::kUnsigned>(lo[k][0], lo[k][1], hi[k][0], hi[k][1], xw[2 * k], xw[2 * k + 1], f);
+        }
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          acc[q][c] = fmaf(f[c] * d[c & 1], c < 2 ? a0 : a1, acc[q][c]);
-          if (kMin) acc[q][c] = fmaf(-(c < 2 ? b0 : b1), xs[c & 1], acc[q][c]);
+        for (int c = 0; c < COLS; ++c) {
+          const float d = __uint_as_float(k ? mt[c].z : mt[c].x), sum = __uint_as_float(k ? mt[c].w : mt[c].y);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float& v = acc[q][2 * i + c];
+            if (kTwo) {
+              v = fmaf(fmaf(h[2 * i + c], b[k][i], f[2 * i + c] * a[k][i]), d, v);
+            } else {
+              v = fmaf(f[2 * i + c] * d, a[k][i], v);
+              if (kMin) v = fmaf(-b[k][i], d * sum, v);
+            }
+          }
         }
       }
     }
@@ -359,8 +451,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int kBoxRows = PAIR ? kRows / 2 : kRows, kPitch = kBoxRows * 128;
   constexpr int kOut = PAIR ? kRows / 2 : kRows;   // outputs of a tile
   constexpr int kSub = kV / 1024;                  // 128-value parts of a warp's slice
-  // blocks and strides of Q4_K, Q5_K and IQ4_XS are multiples of 4 bytes; the box form's rows start on 16
-  constexpr bool kAL = FORM != kRowForm && fmt_block_bytes(FMT) % 4 == 0;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int nst = (p.k + kV - 1) / kV, groups = p.k / 32, kS = p.stages;
@@ -485,13 +575,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   mx_wait();
   const int cw = warp - 1, half = cw >> 3, ks = cw & 7, g = lane >> 2, t = lane & 3;
   const uint32_t sbase = smem_u32(smem), xbase = smem_u32(xres);
-  // this thread's activations inside a stage: codes of token 8 q + g, meta of tokens 8 q + 2 t and 8 q + 2 t + 1. Columns
-  // past the call's tokens repeat the last one (row form) or hold zeros (boxes), and are never stored.
+  // this thread's activations inside a stage: the codes it loads or supplies the address of (box forms: row lane % 8 and
+  // 16-byte chunk lane / 8 of ldmatrix4), and the meta of tokens 8 q + 2 t and 8 q + 2 t + 1. Columns past the call's
+  // tokens repeat the last one (row form) or hold zeros (boxes), and are never stored.
   uint32_t xoff[NT], moff[NT][2];
 #pragma unroll
   for (int q = 0; q < NT; ++q) {
-    const int tok = 8 * q + g;
-    xoff[q] = FORM == kBox1 ? 4 * t : FORM == kBox ? tok * 128 + 4 * t : min(tok, ntok - 1) * kXSlot + 4 * t;
+    xoff[q] = FORM == kBox1 ? (lane >> 3) * 16 : FORM == kBox ? (8 * q + (lane & 7)) * 128 : min(8 * q + g, ntok - 1) * kXSlot + 4 * t;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int tk = 8 * q + 2 * t + c, tr = min(tk, ntok - 1);
@@ -525,28 +615,36 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int sub = 0; sub < kSub; ++sub) {
           const int part = ks * kSub + sub, gc = gst - 4 * part;   // which 128 values; groups left there
           if (gc <= 0) break;
-          // codes and meta of group 4 part + j
-          auto xa = [&](int q, int j, int hi) {
-            if (FORM == kBox)   // one box per 128 values; chunk 2 j + hi of token row (8 q + g), g = row & 7
-              return xb + part * kT * 128 + (xoff[q] ^ uint32_t(((2 * j + hi) ^ g) << 4));
-            return xb + xoff[q] + part * 128 + 32 * j + 16 * hi;
-          };
-          auto ma = [&](int q, int c, int j) {
-            if (FORM == kBox) {   // one box per 16 groups: 16-byte chunk (group / 2) of token row
-              const int gg = 4 * (part & 3) + j;
-              return xb + (part >> 2) * kT * 128 + moff[q][c] + uint32_t(((gg >> 1) ^ (2 * t + c)) << 4) + 8 * (gg & 1);
+          // words of groups 4 part + 2 pr and + 1: values 4t.. and 16 + 4t.. of each
+          auto xa = [&](int q, int pr, uint32_t (&w)[4]) {
+            if constexpr (FORM == kBox) {   // one box per 128 values
+              ldmatrix4(xb + part * kT * 128 + (xoff[q] ^ uint32_t(((4 * pr + (lane >> 3)) ^ (lane & 7)) << 4)), w[0], w[1],
+                        w[2], w[3]);
+            } else if constexpr (FORM == kBox1) {
+              ldmatrix4(xb + xoff[q] + part * 128 + 64 * pr, w[0], w[1], w[2], w[3]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) w[i] = lds(xb + xoff[q] + part * 128 + 64 * pr + 16 * i);
             }
-            return xb + moff[q][c] + part * 32 + 8 * j;
           };
-          if (FORM == kRowForm) {
-            const RowAt r0{sb + (16 * half + g) * kWSlot + ((a0 + uint32_t(st) * kCB) & 15u)};
-            const RowAt r1{sb + (16 * half + g + 8) * kWSlot + ((a1 + uint32_t(st) * kCB) & 15u)};
-            slice_dot<FMT, kAL, NT>(r0, r1, part, gc, lane, xa, ma, acc);
+          auto ma = [&](int q, int c, int pr) {
+            if constexpr (FORM == kBox)   // one box per 16 groups: 16-byte chunk (group / 2) of the token's row
+              return lds128(xb + (part >> 2) * kT * 128 + moff[q][c] +
+                            uint32_t(((2 * (part & 3) + pr) ^ (2 * t + c)) << 4));
+            if constexpr (FORM == kBox1) return lds128(xb + moff[q][c] + part * 32 + 16 * pr);
+            const uint32_t a = xb + moff[q][c] + part * 32 + 16 * pr;
+            return make_uint4(lds(a), lds(a + 4), lds(a + 8), lds(a + 12));
+          };
+          constexpr int kCols = FORM == kBox1 ? 1 : 2;
+          if constexpr (FORM == kRowForm) {
+            const RowAt at{{sb + (16 * half + g) * kWSlot + ((a0 + uint32_t(st) * kCB) & 15u),
+                            sb + (16 * half + g + 8) * kWSlot + ((a1 + uint32_t(st) * kCB) & 15u)}};
+            slice_dot<FMT, NT, kCols>(at, part, gc, lane, xa, ma, acc);
           } else {
-            const uint32_t off = uint32_t(int64_t(st) * kCB) & 127u;
-            const uint32_t base = sb + (PAIR ? half * (kWB / 2) : half * 16 * 128) + g * 128;
-            const BoxAt<kPitch> r0{base, off, uint32_t(g) << 4}, r1{base + 8 * 128, off, uint32_t(g) << 4};
-            slice_dot<FMT, kAL, NT>(r0, r1, part, gc, lane, xa, ma, acc);
+            const uint32_t base = sb + (PAIR ? half * (kWB / 2) : half * 16 * 128);
+            const BoxAt<kPitch> at{base + g * 128, uint32_t(int64_t(st) * kCB) & 127u, uint32_t(g) << 4,
+                                   base + (lane & 15) * 128, uint32_t(lane & 7) << 4, uint32_t(lane >> 4) << 4};
+            slice_dot<FMT, NT, kCols>(at, part, gc, lane, xa, ma, acc);
           }
         }
         __syncwarp();
