@@ -8,8 +8,11 @@
 // 16 + i: one word gives a thread its low and its high half), so a weight is unpacked once for all tokens of the call.
 //
 // A CTA walks tiles of 32 weight rows (of a pair: 16 gate and 16 up rows) over all of k in stages. A producer fills a
-// ring; 16 consumer warps take a row half and one of 8 k slices, so a warp's f32 sums are 4 per 8 tokens, and meet at the
-// tile's end in shared memory. There every output is finished by one thread, in a fixed order of sums.
+// ring; 8 consumer warps take a k slice each, all 32 rows of it, and their f32 sums meet at the tile's end in shared
+// memory. There every output is finished by one thread, in a fixed order of sums.
+//
+// The minima of Q4_K and Q5_K, sum_g dmin m[n][g] * d[t][g] sum_c[t][g], are a product over groups of their own: mma
+// m16n8k4 with the 6-bit m (exact in tf32) and d * sum as the sum of two tf32 parts (22 bits), then one FMA by dmin.
 //
 // Two ways into shared memory. Box form (rows, codes and meta at 16-byte strides): TMA boxes of 128 bytes x 32 rows in
 // the 128-byte swizzle, which puts the 8 rows x 4 words a warp reads at once into 32 banks; the activations stay in
@@ -31,7 +34,7 @@ namespace {
 
 constexpr int kRows = 32;              // weight rows of a tile
 constexpr int kSlices = 8;             // k slices of a stage
-constexpr int kCWarps = 2 * kSlices;   // consumer warps
+constexpr int kCWarps = kSlices;       // consumer warps
 constexpr int kThreads = 32 * (1 + kCWarps);
 constexpr int kTokStride = 36;         // floats between tokens of the partial sums: conflict-free stores
 constexpr int kSmemMax = 227 * 1024;
@@ -106,28 +109,28 @@ LK_DEV void ldmatrix4(uint32_t a, uint32_t& m0, uint32_t& m1, uint32_t& m2, uint
                : "r"(a));
 }
 
-// Where byte b of a stage of this thread's two tile rows (g and g + 8) sits in shared memory, and loads of both.
-// Row form: linear from each row's window, at any 2-byte alignment.
+// Where byte b of a stage of this thread's four tile rows (g, g + 8, g + 16, g + 24) sits in shared memory, and loads of
+// all four. Row form: linear from each row's window, at any 2-byte alignment.
 struct RowAt {
   static constexpr bool kBoxes = false;
-  uint32_t p[2];
-  LK_DEV static uint32_t one(uint32_t a) {
-    const uint32_t c = a & ~3u;
-    return __funnelshift_r(lds(c), lds(c + 4), (a & 3u) * 8u);
-  }
+  uint32_t p[4];
   template <int LOW>
-  LK_DEV void word(uint32_t b, uint32_t& u, uint32_t& v) const {
-    u = one(p[0] + b);
-    v = one(p[1] + b);
+  LK_DEV void word(uint32_t b, uint32_t (&u)[4]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t a = p[i] + b, c = a & ~3u;
+      u[i] = __funnelshift_r(lds(c), lds(c + 4), (a & 3u) * 8u);
+    }
   }
-  LK_DEV void half(uint32_t b, uint32_t& u, uint32_t& v) const {
-    u = lds16(p[0] + b);
-    v = lds16(p[1] + b);
+  LK_DEV void half(uint32_t b, uint32_t (&u)[4]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = lds16(p[i] + b);
   }
 };
-// Box form: 128-byte segments, PITCH bytes apart, of swizzled rows (16-byte chunk c of row r at c ^ (r & 7)); row g + 8
-// is 1024 bytes on with the same swizzle
-template <int PITCH>
+// Box form: 128-byte segments, PITCH bytes apart, of swizzled rows (16-byte chunk c of row r at c ^ (r & 7)). Row g + 8 is
+// 1024 bytes on, rows g + 16 and g + 24 UP bytes (the second half of the box, or the up weight's box), all with the same
+// swizzle, so one address serves four rows.
+template <int PITCH, int UP>
 struct BoxAt {
   static constexpr bool kBoxes = true;
   uint32_t p, off, x;      // row g in segment 0; the stage's first byte in it; (g & 7) << 4
@@ -136,62 +139,74 @@ struct BoxAt {
     b += off;
     return p + (b >> 7) * PITCH + ((b & 0x7Fu) ^ x);
   }
-  // rows g and g + 8 of the 16-byte chunks at b (words t in u0, v0) and b + 16 (u1, v1)
-  LK_DEV void chunks(uint32_t b, uint32_t& u0, uint32_t& v0, uint32_t& u1, uint32_t& v1) const {
+  LK_DEV static constexpr uint32_t row_offset(int i) { return (i & 1) * 1024 + (i >> 1) * UP; }
+  LK_DEV static void four(uint32_t a, uint32_t (&u)[4]) {
+    u[0] = lds(a);
+    u[1] = lds(a + 1024);
+    u[2] = lds(a + UP);
+    u[3] = lds(a + UP + 1024);
+  }
+  // words t of the 16-byte chunks at b (u) and b + 16 (v)
+  LK_DEV void chunks(uint32_t b, uint32_t (&u)[4], uint32_t (&v)[4]) const {
     b += off + mb;
-    ldmatrix4(mp + (b >> 7) * PITCH + ((b & 0x7Fu) ^ mx), u0, v0, u1, v1);
+    const uint32_t a = mp + (b >> 7) * PITCH + ((b & 0x7Fu) ^ mx);
+    ldmatrix4(a, u[0], u[1], v[0], v[1]);
+    ldmatrix4(a + UP, u[2], u[3], v[2], v[3]);
   }
   // LOW: b mod 4 where it is known, else -1 (even)
   template <int LOW>
-  LK_DEV void word(uint32_t b, uint32_t& u, uint32_t& v) const {
+  LK_DEV void word(uint32_t b, uint32_t (&u)[4]) const {
     if (LOW == 0) {
-      const uint32_t a = at(b);
-      u = lds(a);
-      v = lds(a + 1024);
+      four(at(b), u);
       return;
     }
-    const uint32_t lo = at(b & ~3u), hi = at((b & ~3u) + 4), sh = LOW == 2 ? 16u : (b & 3u) * 8u;
-    u = __funnelshift_r(lds(lo), lds(hi), sh);
-    v = __funnelshift_r(lds(lo + 1024), lds(hi + 1024), sh);
+    uint32_t lo[4], hi[4];
+    four(at(b & ~3u), lo);
+    four(at((b & ~3u) + 4), hi);
+    const uint32_t sh = LOW == 2 ? 16u : (b & 3u) * 8u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = __funnelshift_r(lo[i], hi[i], sh);
   }
-  LK_DEV void half(uint32_t b, uint32_t& u, uint32_t& v) const {
+  LK_DEV void half(uint32_t b, uint32_t (&u)[4]) const {
     const uint32_t a = at(b);
-    u = lds16(a);
-    v = lds16(a + 1024);
+    u[0] = lds16(a);
+    u[1] = lds16(a + 1024);
+    u[2] = lds16(a + UP);
+    u[3] = lds16(a + UP + 1024);
   }
 };
 
-// 128 values (4 groups) of a thread's two tile rows: the packed words it contributes to the MMAs (t = lane & 3). For
+// 128 values (4 groups) of a thread's four tile rows: the packed words it contributes to the MMAs (t = lane & 3). For
 // group j and row i, lo holds the codes of values 4t .. 4t + 3 and hi those of 16 + 4t .. 16 + 4t + 3, one per byte, u8 or
 // s8, times the power of two that its scale divides by.
 template <int FMT>
 struct Slice {
   static constexpr bool kUnsigned = FMT == LK_Q4_K || FMT == LK_Q5_K;
   static constexpr int kQk = fmt_qk(FMT), kBb = fmt_block_bytes(FMT);
-  // b mod 4 of a field at byte c of block j: known for blocks of an even number of 4-byte words, or where j is
+  // byte c of block j, mod 4 (blocks start at a multiple of 8 for j = 0)
   static constexpr int low(int c, int j) { return (j * kBb + c) % 4; }
-  uint32_t r[2][FMT == LK_Q8_0 || FMT == LK_Q5_0 ? 8 : FMT == LK_Q5_K || FMT == LK_Q6_K ? 6 : 4];
+  uint32_t r[FMT == LK_Q8_0 || FMT == LK_Q5_0 ? 8 : FMT == LK_Q5_K || FMT == LK_Q6_K ? 6 : 4][4];   // [word][row]
 
   template <int J, class At>
   LK_DEV void load_block(const At& at, uint32_t b, int t) {
-    if (FMT == LK_Q8_0) {
-      at.template word<low(2, J)>(b + 2 + 4 * t, r[0][2 * J], r[1][2 * J]);
-      at.template word<low(2, J)>(b + 18 + 4 * t, r[0][2 * J + 1], r[1][2 * J + 1]);
-    } else if (FMT == LK_Q5_0) {
-      at.template word<low(6, J)>(b + 6 + 4 * t, r[0][2 * J], r[1][2 * J]);
+    if constexpr (FMT == LK_Q8_0) {
+      at.template word<low(2, J)>(b + 2 + 4 * t, r[2 * J]);
+      at.template word<low(2, J)>(b + 18 + 4 * t, r[2 * J + 1]);
+    } else if constexpr (FMT == LK_Q5_0) {
+      at.template word<low(6, J)>(b + 6 + 4 * t, r[2 * J]);
       // bits 4t .. 4t + 3 and 16 + 4t .. of qh, in one word: bits 0-3 and 16-19
-      at.template word<low(2, J)>(b + 2, r[0][2 * J + 1], r[1][2 * J + 1]);
+      at.template word<low(2, J)>(b + 2, r[2 * J + 1]);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) r[i][2 * J + 1] = (r[i][2 * J + 1] >> (4 * t)) & 0x000F000Fu;
+      for (int i = 0; i < 4; ++i) r[2 * J + 1][i] = (r[2 * J + 1][i] >> (4 * t)) & 0x000F000Fu;
     } else {
-      at.template word<low(2, J)>(b + 2 + 4 * t, r[0][J], r[1][J]);
+      at.template word<low(2, J)>(b + 2 + 4 * t, r[J]);
     }
   }
   // part: which 128 values of the stage
   template <class At>
   LK_DEV void load(const At& at, int part, int t) {
     if constexpr (kQk == 32) {
-      const uint32_t b = 4 * part * kBb;   // a multiple of 8
+      const uint32_t b = 4 * part * kBb;
       load_block<0>(at, b, t);
       load_block<1>(at, b + kBb, t);
       load_block<2>(at, b + 2 * kBb, t);
@@ -201,34 +216,29 @@ struct Slice {
       const int h = part & 1;
       if constexpr ((FMT == LK_Q4_K || FMT == LK_Q5_K) && At::kBoxes) {
         constexpr int kQs = FMT == LK_Q4_K ? 16 : 48;
-        at.chunks(b + kQs + 64 * h, r[0][0], r[1][0], r[0][1], r[1][1]);
-        at.chunks(b + kQs + 64 * h + 32, r[0][2], r[1][2], r[0][3], r[1][3]);
-        if constexpr (FMT == LK_Q5_K) {
-          at.chunks(b + 16, r[0][4], r[1][4], r[0][5], r[1][5]);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            r[i][4] >>= 4 * h;
-            r[i][5] >>= 4 * h;
-          }
-        }
+        at.chunks(b + kQs + 64 * h, r[0], r[1]);
+        at.chunks(b + kQs + 64 * h + 32, r[2], r[3]);
+        if constexpr (FMT == LK_Q5_K) at.chunks(b + 16, r[4], r[5]);
       } else if constexpr (FMT == LK_Q4_K || FMT == LK_Q5_K || FMT == LK_IQ4_XS) {
         constexpr int kQs = FMT == LK_Q4_K ? 16 : FMT == LK_Q5_K ? 48 : 8;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) at.template word<0>(b + kQs + 64 * h + 16 * i + 4 * t, r[0][i], r[1][i]);
+        for (int i = 0; i < 4; ++i) at.template word<0>(b + kQs + 64 * h + 16 * i + 4 * t, r[i]);
         if constexpr (FMT == LK_Q5_K) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            at.template word<0>(b + 16 + 16 * i + 4 * t, r[0][4 + i], r[1][4 + i]);
-            r[0][4 + i] >>= 4 * h;
-            r[1][4 + i] >>= 4 * h;
-          }
+          at.template word<0>(b + 16 + 4 * t, r[4]);
+          at.template word<0>(b + 32 + 4 * t, r[5]);
         }
       } else {   // Q6_K
 #pragma unroll
-        for (int i = 0; i < 4; ++i) at.template word<-1>(b + 64 * h + 16 * i + 4 * t, r[0][i], r[1][i]);
+        for (int i = 0; i < 4; ++i) at.template word<-1>(b + 64 * h + 16 * i + 4 * t, r[i]);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          at.template word<-1>(b + 128 + 32 * h + 16 * i + 4 * t, r[0][4 + i], r[1][4 + i]);
+        for (int i = 0; i < 2; ++i) at.template word<-1>(b + 128 + 32 * h + 16 * i + 4 * t, r[4 + i]);
+      }
+      if constexpr (FMT == LK_Q5_K) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          r[4][i] >>= 4 * h;
+          r[5][i] >>= 4 * h;
+        }
       }
     }
   }
@@ -236,93 +246,109 @@ struct Slice {
   // the codes of group j (0..3) of row i
   LK_DEV void codes(int i, int j, uint32_t& lo, uint32_t& hi) const {
     constexpr uint32_t kLow = 0x0F0F0F0Fu, kHigh = 0xF0F0F0F0u, kTop = 0x80808080u;
-    const uint32_t* w = r[i];
     if constexpr (FMT == LK_Q4_0) {            // 16 (q - 8)
-      lo = ((w[j] << 4) & kHigh) ^ kTop;
-      hi = (w[j] & kHigh) ^ kTop;
+      lo = ((r[j][i] << 4) & kHigh) ^ kTop;
+      hi = (r[j][i] & kHigh) ^ kTop;
     } else if constexpr (FMT == LK_IQ4_NL || FMT == LK_IQ4_XS) {
-      lo = iq4_lookup4(w[j] & kLow) ^ kTop;
-      hi = iq4_lookup4((w[j] >> 4) & kLow) ^ kTop;
+      lo = iq4_lookup4(r[j][i] & kLow) ^ kTop;
+      hi = iq4_lookup4((r[j][i] >> 4) & kLow) ^ kTop;
     } else if constexpr (FMT == LK_Q8_0) {
-      lo = w[2 * j];
-      hi = w[2 * j + 1];
+      lo = r[2 * j][i];
+      hi = r[2 * j + 1][i];
     } else if constexpr (FMT == LK_Q5_0) {     // 8 (q - 16): the nibble at bit 3, the fifth bit at 7
-      const uint32_t q = w[2 * j], b = w[2 * j + 1];
+      const uint32_t q = r[2 * j][i], b = r[2 * j + 1][i];
       lo = (((q & kLow) << 3) | spread(b)) ^ kTop;
       hi = (((q >> 1) & 0x78787878u) | spread(b >> 16)) ^ kTop;
     } else if constexpr (FMT == LK_Q4_K) {     // page j / 2: even groups q, odd groups 16 q
       const uint32_t m = (j & 1) ? kHigh : kLow;
-      lo = w[2 * (j >> 1)] & m;
-      hi = w[2 * (j >> 1) + 1] & m;
+      lo = r[2 * (j >> 1)][i] & m;
+      hi = r[2 * (j >> 1) + 1][i] & m;
     } else if constexpr (FMT == LK_Q5_K) {     // nibble | bit j << 4
-      lo = ((w[2 * (j >> 1)] >> (4 * (j & 1))) & kLow) | (((w[4] >> j) & 0x01010101u) << 4);
-      hi = ((w[2 * (j >> 1) + 1] >> (4 * (j & 1))) & kLow) | (((w[5] >> j) & 0x01010101u) << 4);
+      lo = ((r[2 * (j >> 1)][i] >> (4 * (j & 1))) & kLow) | (((r[4][i] >> j) & 0x01010101u) << 4);
+      hi = ((r[2 * (j >> 1) + 1][i] >> (4 * (j & 1))) & kLow) | (((r[5][i] >> j) & 0x01010101u) << 4);
     } else {                                   // Q6_K: 4 (q - 32): nibble at bit 2, the two high bits at 6
-      lo = six(w[2 * (j & 1)], w[4], j);
-      hi = six(w[2 * (j & 1) + 1], w[5], j);
+      lo = six(r[2 * (j & 1)][i], r[4][i], j);
+      hi = six(r[2 * (j & 1) + 1][i], r[5][i], j);
     }
   }
-  // factor of the codes' scale
-  [[maybe_unused]] static constexpr float kInv0 = FMT == LK_Q4_0 ? 0.0625f : FMT == LK_Q5_0 ? 0.125f : FMT == LK_Q6_K ? 0.25f : 1.0f;
-  [[maybe_unused]] static constexpr float kInv1 = FMT == LK_Q4_K ? 0.0625f : kInv0;   // odd groups
+  // factor of the codes' scale, of even and of odd groups
+  static constexpr float inv(int odd) {
+    return FMT == LK_Q4_0 || (FMT == LK_Q4_K && odd) ? 0.0625f : FMT == LK_Q5_0 ? 0.125f : FMT == LK_Q6_K ? 0.25f : 1.0f;
+  }
 
-  // scales s of group t of both rows, and their minima (Q4_K, Q5_K) or second 16 values' scales (Q6_K) in m: this lane's
-  // share of what the four lanes of a row exchange
+  // This lane's share of what the four lanes of a row exchange: scales s of group t of its four rows, and in m the second
+  // 16 values' scales (Q6_K) or the 6-bit minima (Q4_K, Q5_K; dmin: their rows' factor).
   template <class At>
-  LK_DEV static void scales(const At& at, int part, int t, float (&s)[2], float (&m)[2]) {
-    m[0] = m[1] = 0.0f;
-    uint32_t d[2];
+  LK_DEV static void scales(const At& at, int part, int t, float (&s)[4], float (&m)[4], float (&dmin)[4]) {
+    uint32_t d[4];
     if constexpr (kQk == 32) {
-      at.half((4 * part + t) * kBb, d[0], d[1]);
+      at.half((4 * part + t) * kBb, d);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) s[i] = h2f(uint16_t(d[i])) * kInv0;
-      return;
-    }
-    const uint32_t b = (part >> 1) * kBb;
-    const int j = 4 * (part & 1) + t;
-    if constexpr (FMT == LK_Q4_K || FMT == LK_Q5_K) {
-      uint4 h[2];
-      if constexpr (At::kBoxes) {
-        const uint32_t a = at.at(b);
-        h[0] = lds128(a);
-        h[1] = lds128(a + 1024);
-      } else {
-        at.template word<0>(b, h[0].x, h[1].x);
-        at.template word<0>(b + 4, h[0].y, h[1].y);
-        at.template word<0>(b + 8, h[0].z, h[1].z);
-        at.template word<0>(b + 12, h[0].w, h[1].w);
-      }
+      for (int i = 0; i < 4; ++i) s[i] = h2f(uint16_t(d[i])) * inv(0);
+    } else {
+      const uint32_t b = (part >> 1) * kBb;
+      const int h = part & 1, j = 4 * h + t;
+      if constexpr (FMT == LK_Q4_K || FMT == LK_Q5_K) {
+        uint32_t s0[4], s1[4], s2[4];
+        if constexpr (At::kBoxes) {
+          const uint32_t a = at.at(b);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        uint32_t sc, mn;
-        q4k_scale_min_w(h[i].y, h[i].z, h[i].w, j, sc, mn);
-        s[i] = h2f(uint16_t(h[i].x & 0xffffu)) * float(sc) * ((t & 1) ? kInv1 : kInv0);
-        m[i] = h2f(uint16_t(h[i].x >> 16)) * float(mn);
-      }
-    } else if constexpr (FMT == LK_Q6_K) {
-      uint32_t two[2];
-      at.half(b + 192 + 2 * j, two[0], two[1]);
-      at.half(b + 208, d[0], d[1]);
+          for (int i = 0; i < 4; ++i) {
+            const uint4 q = lds128(a + at.row_offset(i));
+            d[i] = q.x;
+            s0[i] = q.y;
+            s1[i] = q.z;
+            s2[i] = q.w;
+          }
+        } else {
+          at.template word<0>(b, d);
+          at.template word<0>(b + 4, s0);
+          at.template word<0>(b + 8, s1);
+          at.template word<0>(b + 12, s2);
+        }
+        const float f = (t & 1) ? inv(1) : inv(0);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float f = h2f(uint16_t(d[i])) * kInv0;
-        s[i] = f * float(int8_t(two[i] & 255u));
-        m[i] = f * float(int8_t(two[i] >> 8));
-      }
-    } else {   // IQ4_XS
-      uint32_t sh[2], sl[2];
-      at.half(b, d[0], d[1]);
-      at.half(b + 2, sh[0], sh[1]);
-      at.template word<0>(b + 4, sl[0], sl[1]);
+        for (int i = 0; i < 4; ++i) {
+          // q4k_scale_min_w with the half h, uniform in a warp, outside
+          uint32_t sc = s0[i] >> (8 * t), mn = s1[i] >> (8 * t);
+          if (h == 0) {
+            sc &= 63u;
+            mn &= 63u;
+          } else {
+            const uint32_t lo = s2[i] >> (8 * t);
+            sc = (lo & 15u) | ((sc >> 2) & 48u);
+            mn = ((lo >> 4) & 15u) | ((mn >> 2) & 48u);
+          }
+          s[i] = h2f(uint16_t(d[i] & 0xffffu)) * u2f(sc) * f;
+          m[i] = u2f(mn);
+          dmin[i] = h2f(uint16_t(d[i] >> 16));
+        }
+      } else if constexpr (FMT == LK_Q6_K) {
+        uint32_t two[4];
+        at.half(b + 192 + 2 * j, two);
+        at.half(b + 208, d);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int ls = int(((sl[i] >> (4 * j)) & 15u) | (((sh[i] >> (2 * j)) & 3u) << 4));
-        s[i] = h2f(uint16_t(d[i])) * float(ls - 32);
+        for (int i = 0; i < 4; ++i) {
+          const float f = h2f(uint16_t(d[i])) * inv(0);
+          s[i] = f * float(int8_t(two[i] & 255u));
+          m[i] = f * float(int8_t(two[i] >> 8));
+        }
+      } else {   // IQ4_XS
+        uint32_t sh[4], sl[4];
+        at.half(b, d);
+        at.half(b + 2, sh);
+        at.template word<0>(b + 4, sl);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int ls = int(((sl[i] >> (4 * j)) & 15u) | (((sh[i] >> (2 * j)) & 3u) << 4));
+          s[i] = h2f(uint16_t(d[i])) * float(ls - 32);
+        }
       }
     }
   }
 
  private:
+  LK_DEV static float u2f(uint32_t v) { return __uint_as_float(0x4B000000u | v) - 8388608.0f; }   // v < 2^23, exact
   // bits 0..3 -> bit 7 of bytes 0..3
   LK_DEV static uint32_t spread(uint32_t b) { return ((b & 15u) * 0x10204080u) & 0x80808080u; }
   LK_DEV static uint32_t six(uint32_t ql, uint32_t qh, int j) {
@@ -373,29 +399,55 @@ LK_DEV void store_q8(uint8_t* y, int64_t total, int64_t at, float v, int lane) {
     reinterpret_cast<float2*>(y + total)[at / 32] = make_float2(__half2float(__float2half_rn(d)), float(sum));
 }
 
-// 4 groups of 16 rows x 8 NT tokens: the warp's sums grow by the groups' dots. x(q, pr, w): the codes' words of groups
-// 2 pr and 2 pr + 1 for token 8 q + g; m(q, c, pr): (scale, sum of codes) of those groups for token 8 q + 2 t + c. COLS: the
-// columns a thread keeps (1 where the call has one token).
-template <int FMT, int NT, int COLS, class At, class XAt, class MAt>
-LK_DEV void slice_dot(const At& at, int part, int gc, int lane, const XAt& x, const MAt& m, float (&acc)[NT][4]) {
+// D += A . B of 16 x 4 by 4 x 8 in tf32 (the low 13 bits of the operands are not read)
+LK_DEV void mma_tf32(float a0, float a1, float b, float (&d)[4]) {
+  asm("mma.sync.aligned.m16n8k4.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(__float_as_uint(a0)), "r"(__float_as_uint(a1)), "r"(__float_as_uint(b)));
+}
+
+// 4 groups of 32 rows x 8 NT tokens: the warp's sums grow by the groups' dots. acc[q][4 h + 2 i + c]: row 16 h + 8 i + g,
+// token 8 q + 2 t + c. x(q, pr, w): the codes' words of groups 2 pr and 2 pr + 1 for token 8 q + g; m(q, c, pr): (scale, sum of
+// codes) of those groups for token 8 q + 2 t + c; xs(q): of group t for token 8 q + g. COLS: the columns a thread keeps (1
+// where the call has one token).
+template <int FMT, int NT, int COLS, class At, class XAt, class MAt, class SAt>
+LK_DEV void slice_dot(const At& at, int part, int gc, int lane, const XAt& x, const MAt& m, const SAt& xs,
+                      float (&acc)[NT][8]) {
   constexpr bool kTwo = FMT == LK_Q6_K, kMin = FMT == LK_Q4_K || FMT == LK_Q5_K;
   const int t = lane & 3;
   Slice<FMT> w;
   w.load(at, part, t);
-  float s[2], z[2];
-  Slice<FMT>::scales(at, part, t, s, z);
+  float s[4], z[4], dmin[4];
+  Slice<FMT>::scales(at, part, t, s, z, dmin);
+  if (kMin) {   // k is whole super-blocks: all 4 groups
+#pragma unroll
+    for (int q = 0; q < NT; ++q) {
+      const float v = xs(q), hi = __uint_as_float(__float_as_uint(v) & 0xFFFFE000u), lo = v - hi;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float p[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        mma_tf32(z[2 * h], z[2 * h + 1], hi, p);
+        mma_tf32(z[2 * h], z[2 * h + 1], lo, p);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int c = 0; c < COLS; ++c)
+            acc[q][4 * h + 2 * i + c] = fmaf(-dmin[2 * h + i], p[2 * i + c], acc[q][4 * h + 2 * i + c]);
+      }
+    }
+  }
 #pragma unroll
   for (int pr = 0; pr < 2; ++pr) {
     if (2 * pr >= gc) break;
-    uint32_t lo[2][2], hi[2][2];   // [group][row]
-    float a[2][2], b[2][2];
+    uint32_t lo[2][4], hi[2][4];   // [group][row]
+    float a[2][4], b[2][4];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int j = 2 * pr + k, from = (lane & 28) | j;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < 4; ++i) {
         a[k][i] = __shfl_sync(0xFFFFFFFFu, s[i], from);
-        if (kTwo || kMin) b[k][i] = __shfl_sync(0xFFFFFFFFu, z[i], from);
+        if (kTwo) b[k][i] = __shfl_sync(0xFFFFFFFFu, z[i], from);
         w.codes(i, j, lo[k][i], hi[k][i]);
       }
     }
@@ -409,24 +461,25 @@ LK_DEV void slice_dot(const At& at, int part, int gc, int lane, const XAt& x, co
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         if (!At::kBoxes && 2 * pr + k >= gc) break;   // box form: an even number of groups
-        float f[4], h[4];
-        if (kTwo) {
-          mma_k16(lo[k][0], lo[k][1], xw[2 * k], f);
-          mma_k16(hi[k][0], hi[k][1], xw[2 * k + 1], h);
-        } else {
-          mma_k32<Slice<FMT>::kUnsigned>(lo[k][0], lo[k][1], hi[k][0], hi[k][1], xw[2 * k], xw[2 * k + 1], f);
-        }
 #pragma unroll
-        for (int c = 0; c < COLS; ++c) {
-          const float d = __uint_as_float(k ? mt[c].z : mt[c].x), sum = __uint_as_float(k ? mt[c].w : mt[c].y);
+        for (int h = 0; h < 2; ++h) {
+          float f[4], e[4];
+          if (kTwo) {
+            mma_k16(lo[k][2 * h], lo[k][2 * h + 1], xw[2 * k], f);
+            mma_k16(hi[k][2 * h], hi[k][2 * h + 1], xw[2 * k + 1], e);
+          } else {
+            mma_k32<Slice<FMT>::kUnsigned>(lo[k][2 * h], lo[k][2 * h + 1], hi[k][2 * h], hi[k][2 * h + 1], xw[2 * k],
+                                           xw[2 * k + 1], f);
+          }
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float& v = acc[q][2 * i + c];
-            if (kTwo) {
-              v = fmaf(fmaf(h[2 * i + c], b[k][i], f[2 * i + c] * a[k][i]), d, v);
-            } else {
-              v = fmaf(f[2 * i + c] * d, a[k][i], v);
-              if (kMin) v = fmaf(-b[k][i], d * sum, v);
+          for (int c = 0; c < COLS; ++c) {
+            const float d = __uint_as_float(k ? mt[c].z : mt[c].x);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float& v = acc[q][4 * h + 2 * i + c];
+              const int r = 2 * h + i;
+              if (kTwo) v = fmaf(fmaf(e[2 * i + c], b[k][r], f[2 * i + c] * a[k][r]), d, v);
+              else v = fmaf(f[2 * i + c] * d, a[k][r], v);
             }
           }
         }
@@ -573,12 +626,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // ------------------------------------------------------------------ consumers
   mx_wait();
-  const int cw = warp - 1, half = cw >> 3, ks = cw & 7, g = lane >> 2, t = lane & 3;
+  const int ks = warp - 1, g = lane >> 2, t = lane & 3;
   const uint32_t sbase = smem_u32(smem), xbase = smem_u32(xres);
   // this thread's activations inside a stage: the codes it loads or supplies the address of (box forms: row lane % 8 and
   // 16-byte chunk lane / 8 of ldmatrix4), and the meta of tokens 8 q + 2 t and 8 q + 2 t + 1. Columns past the call's
   // tokens repeat the last one (row form) or hold zeros (boxes), and are never stored.
-  uint32_t xoff[NT], moff[NT][2];
+  uint32_t xoff[NT], moff[NT][2], soff[NT];
 #pragma unroll
   for (int q = 0; q < NT; ++q) {
     xoff[q] = FORM == kBox1 ? (lane >> 3) * 16 : FORM == kBox ? (8 * q + (lane & 7)) * 128 : min(8 * q + g, ntok - 1) * kXSlot + 4 * t;
@@ -588,6 +641,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t a = uint32_t(reinterpret_cast<uintptr_t>(p.meta)) + uint32_t(t0 + tr) * uint32_t(groups) * 8u;
       moff[q][c] = FORM == kBox1 ? kV : FORM == kBox ? kT * kV + tk * 128 : kT * kXSlot + tr * kMetaSlot + (a & 15u);
     }
+    // the meta of group t of token 8 q + g
+    const int tr = min(8 * q + g, ntok - 1);
+    const uint32_t a = uint32_t(reinterpret_cast<uintptr_t>(p.meta)) + uint32_t(t0 + tr) * uint32_t(groups) * 8u;
+    soff[q] = FORM == kBox1 ? kV + 8 * t : FORM == kBox ? kT * kV + (8 * q + g) * 128 + 8 * (t & 1)
+                                                        : kT * kXSlot + tr * kMetaSlot + (a & 15u) + 8 * t;
   }
   int s = 0;
   uint32_t turn = 0;
@@ -596,13 +654,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < p.tiles_per_unit && live; ++i) {
       const int tile = u * p.tiles_per_unit + i;
       if (tile >= ntile) break;
-      float acc[NT][4];
+      float acc[NT][8];
 #pragma unroll
       for (int q = 0; q < NT; ++q)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) acc[q][c] = 0.0f;
-      // row form: low address bits of the two rows' windows
-      const uint32_t a0 = uint32_t(row_src(tile, 16 * half + g, 0)), a1 = uint32_t(row_src(tile, 16 * half + g + 8, 0));
+        for (int c = 0; c < 8; ++c) acc[q][c] = 0.0f;
+      uint32_t low[4];   // row form: low address bits of the four rows' windows
+#pragma unroll
+      for (int r = 0; r < 4; ++r) low[r] = FORM == kRowForm ? uint32_t(row_src(tile, 8 * r + g, 0)) : 0u;
       for (int st = 0; st < nst; ++st) {
         if (!__all_sync(0xFFFFFFFFu, poll(&full[s], turn))) {
           atomicOr(&g_status, 1u);
@@ -611,7 +670,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const uint32_t sb = sbase + s * slot, xb = p.resident ? xbase + st * kXB : sb + kWB;
         const int gst = min(kV / 32, groups - st * (kV / 32));
-#pragma unroll
+#pragma unroll 1
         for (int sub = 0; sub < kSub; ++sub) {
           const int part = ks * kSub + sub, gc = gst - 4 * part;   // which 128 values; groups left there
           if (gc <= 0) break;
@@ -635,16 +694,22 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t a = xb + moff[q][c] + part * 32 + 16 * pr;
             return make_uint4(lds(a), lds(a + 4), lds(a + 8), lds(a + 12));
           };
+          auto sa = [&](int q) {
+            const uint32_t a = FORM == kBox ? xb + (part >> 2) * kT * 128 + soff[q] + uint32_t(((2 * (part & 3) + (t >> 1)) ^ g) << 4)
+                                            : xb + soff[q] + part * 32;
+            return __uint_as_float(lds(a)) * __uint_as_float(lds(a + 4));
+          };
           constexpr int kCols = FORM == kBox1 ? 1 : 2;
           if constexpr (FORM == kRowForm) {
-            const RowAt at{{sb + (16 * half + g) * kWSlot + ((a0 + uint32_t(st) * kCB) & 15u),
-                            sb + (16 * half + g + 8) * kWSlot + ((a1 + uint32_t(st) * kCB) & 15u)}};
-            slice_dot<FMT, NT, kCols>(at, part, gc, lane, xa, ma, acc);
+            RowAt at;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) at.p[r] = sb + (8 * r + g) * kWSlot + ((low[r] + uint32_t(st) * kCB) & 15u);
+            slice_dot<FMT, NT, kCols>(at, part, gc, lane, xa, ma, sa, acc);
           } else {
-            const uint32_t base = sb + (PAIR ? half * (kWB / 2) : half * 16 * 128);
-            const BoxAt<kPitch> at{base + g * 128, uint32_t(int64_t(st) * kCB) & 127u, uint32_t(g) << 4,
-                                   base + (lane & 15) * 128, uint32_t(lane & 7) << 4, uint32_t(lane >> 4) << 4};
-            slice_dot<FMT, NT, kCols>(at, part, gc, lane, xa, ma, acc);
+            const BoxAt<kPitch, PAIR ? kWB / 2 : 16 * 128> at{sb + g * 128, uint32_t(int64_t(st) * kCB) & 127u,
+                                                              uint32_t(g) << 4, sb + (lane & 15) * 128,
+                                                              uint32_t(lane & 7) << 4, uint32_t(lane >> 4) << 4};
+            slice_dot<FMT, NT, kCols>(at, part, gc, lane, xa, ma, sa, acc);
           }
         }
         __syncwarp();
@@ -656,13 +721,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!__all_sync(0xFFFFFFFFu, live)) live = false;
       // the slices' sums meet: [slice][token][row]
-      asm volatile("bar.sync 1, 512;" ::: "memory");   // the last tile's have been read
+      asm volatile("bar.sync 1, 256;" ::: "memory");   // the last tile's have been read
 #pragma unroll
       for (int q = 0; q < NT; ++q)
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-          red[(ks * kT + 8 * q + 2 * t + (c & 1)) * kTokStride + 16 * half + g + (c >= 2 ? 8 : 0)] = acc[q][c];
-      asm volatile("bar.sync 1, 512;" ::: "memory");
+        for (int c = 0; c < 8; ++c)
+          red[(ks * kT + 8 * q + 2 * t + (c & 1)) * kTokStride + 8 * (c >> 1) + g] = acc[q][c];
+      asm volatile("bar.sync 1, 256;" ::: "memory");
       const int ctid = threadIdx.x - 32;
       for (int o = ctid; o < kT * kOut; o += 32 * kCWarps) {   // whole warps: kOut * 8 is a multiple of 32
         const int tk = o / kOut, r = o % kOut, n = tile * kOut + r;
