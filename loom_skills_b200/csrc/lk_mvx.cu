@@ -7,9 +7,10 @@
 // token as for 8, and the packed 4-bit words are already in its operand order (byte i of a block holds values i and
 // 16 + i: one word gives a thread its low and its high half), so a weight is unpacked once for all tokens of the call.
 //
-// A CTA walks tiles of 32 weight rows (of a pair: 16 gate and 16 up rows) over all of k in stages. A producer fills a
-// ring; 8 consumer warps take a k slice each, all 32 rows of it, and their f32 sums meet at the tile's end in shared
-// memory. There every output is finished by one thread, in a fixed order of sums.
+// A CTA walks tiles of weight rows over all of k in stages. A producer fills a ring; 16 consumer warps are two groups of
+// 8, a warp taking 32 rows (of a pair: 16 gate and 16 up rows) of one of 8 k slices. Many tiles: a tile is 64 rows, each
+// group takes 32 of them. At most one tile an SM: a tile is 32 rows and the groups take its stages in turn. The warps'
+// f32 sums meet at the tile's end in shared memory, where one thread finishes each output, in a fixed order of sums.
 //
 // The minima of Q4_K and Q5_K, sum_g dmin m[n][g] * d[t][g] sum_c[t][g], are a product over groups of their own: mma
 // m16n8k4 with the 6-bit m (exact in tf32) and d * sum as the sum of two tf32 parts (22 bits), then one FMA by dmin.
@@ -32,9 +33,9 @@ int make_map(CUtensorMap* map, const void* base, CUtensorMapDataType dt, int ele
 
 namespace {
 
-constexpr int kRows = 32;              // weight rows of a tile
-constexpr int kSlices = 8;             // k slices of a stage
-constexpr int kCWarps = kSlices;       // consumer warps
+constexpr int kRows = 32;              // weight rows of a warp
+constexpr int kSlices = 8;             // k slices of a stage, a warp of each group for each
+constexpr int kCWarps = 2 * kSlices;   // consumer warps
 constexpr int kThreads = 32 * (1 + kCWarps);
 constexpr int kTokStride = 36;         // floats between tokens of the partial sums: conflict-free stores
 constexpr int kSmemMax = 227 * 1024;
@@ -47,8 +48,8 @@ LK_DEV void mx_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "
 // How a call's operands reach shared memory, and its tokens: kBox1 is the box form of one token, whose codes need no
 // swizzle (all rows read the same words) and come by plain bulk copies.
 enum { kRowForm = 0, kBox = 1, kBox1 = 2 };
-// values of a stage: 2048 for up to 8 tokens, else 1024 (the same in every form, so that all sum in the same order)
-__host__ __device__ constexpr int stage_values(int nt) { return nt == 1 ? 2048 : 1024; }
+// values of a stage (rg: the row groups of a tile, 1 or 2); the same in every form, so that all sum in the same order
+__host__ __device__ constexpr int stage_values(int rg, int nt) { return rg == 1 && nt == 1 ? 2048 : 1024; }
 // packed bytes of a row's stage; 128-byte segments that can hold them wherever they start
 __host__ __device__ constexpr int stage_bytes(int fmt, int v) { return v / fmt_qk(fmt) * fmt_block_bytes(fmt); }
 __host__ __device__ constexpr int segments(int fmt, int v) {
@@ -59,14 +60,22 @@ __host__ __device__ constexpr int segments(int fmt, int v) {
 __host__ __device__ constexpr int slot_of(int bytes) { return (bytes + 32 + 111) / 128 * 128 + 16; }
 // weight bytes of a stage in shared memory, and a stage's activations (box forms: multiples of 1024, which the swizzle's
 // pattern is aligned to)
-__host__ __device__ constexpr int w_bytes(int fmt, int form, int v) {
-  return form == kRowForm ? kRows * slot_of(stage_bytes(fmt, v)) : segments(fmt, v) * kRows * 128;
+__host__ __device__ constexpr int w_bytes(int fmt, int form, int rg, int v) {
+  return rg * kRows * (form == kRowForm ? slot_of(stage_bytes(fmt, v)) : segments(fmt, v) * 128);
 }
 __host__ __device__ constexpr int x_bytes(int form, int nt, int v) {
   return form == kRowForm ? 8 * nt * (slot_of(v) + slot_of(v / 4)) : form == kBox1 ? (v + v / 4 + 1023) / 1024 * 1024 : 8 * nt * (v + v / 4);
 }
-constexpr int red_bytes(int nt) { return kSlices * 8 * nt * kTokStride * 4; }
+// partial sums of all 16 warps; for 32 tokens of half of them, to which the other half adds
+constexpr int red_slices(int nt) { return nt <= 2 ? kCWarps : kCWarps / 2; }
+constexpr int red_bytes(int nt) { return red_slices(nt) * 8 * nt * kTokStride * 4; }
 constexpr int kTailBytes = 256 + 16 * 32 * 4;   // barriers; the first tile of a unit of two (q8 output of a pair)
+constexpr int fixed_bytes(int nt) { return 1024 + red_bytes(nt) + kTailBytes; }
+// whether two stages of 64-row tiles fit beside the sums
+constexpr bool two_groups(int fmt, int form, int nt) {
+  const int v = stage_values(2, nt);
+  return form != kRowForm && 2 * (w_bytes(fmt, form, 2, v) + x_bytes(form, nt, v)) + fixed_bytes(nt) <= kSmemMax;
+}
 
 struct MvxArgs {
   int n, k, tokens;
@@ -373,7 +382,7 @@ LK_DEV void mma_k32(uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t
         : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(kMagicBits));
 #pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = __int_as_float(c[i]) - kMagic;   // exact: |dot| < 2^22
+  for (int i = 0; i < 4; ++i) f[i] = __int_as_float(c[i]);   // |dot| < 2^22
 }
 LK_DEV void mma_k16(uint32_t a0, uint32_t a1, uint32_t b0, float (&f)[4]) {
   int c[4];
@@ -381,7 +390,7 @@ LK_DEV void mma_k16(uint32_t a0, uint32_t a1, uint32_t b0, float (&f)[4]) {
       : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
       : "r"(a0), "r"(a1), "r"(b0), "r"(kMagicBits));
 #pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = __int_as_float(c[i]) - kMagic;
+  for (int i = 0; i < 4; ++i) f[i] = __int_as_float(c[i]);
 }
 
 // k_quant_q8's codes and meta of one 32-value group, one value a lane
@@ -473,13 +482,15 @@ LK_DEV void slice_dot(const At& at, int part, int gc, int lane, const XAt& x, co
           }
 #pragma unroll
           for (int c = 0; c < COLS; ++c) {
-            const float d = __uint_as_float(k ? mt[c].z : mt[c].x);
+            // dot * d as (12582912 + dot) * d - 12582912 * d: the scale has the 11 bits of an f16, so the second product
+            // is exact and the whole rounds once (an infinite scale gives NaN)
+            const float d = __uint_as_float(k ? mt[c].z : mt[c].x), off = -kMagic * d;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               float& v = acc[q][4 * h + 2 * i + c];
               const int r = 2 * h + i;
-              if (kTwo) v = fmaf(fmaf(e[2 * i + c], b[k][r], f[2 * i + c] * a[k][r]), d, v);
-              else v = fmaf(f[2 * i + c] * d, a[k][r], v);
+              v = fmaf(fmaf(f[2 * i + c], d, off), a[k][r], v);
+              if (kTwo) v = fmaf(fmaf(e[2 * i + c], d, off), b[k][r], v);
             }
           }
         }
@@ -494,15 +505,16 @@ LK_DEV bool poll(uint64_t* bar, uint32_t phase) {
   return false;
 }
 
-template <int FMT, int FORM, bool PAIR, int NT>
+template <int FMT, int FORM, bool PAIR, int NT, int RG>
 __global__ void __launch_bounds__(kThreads, 1)
     k_mvx(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap w2map,
           const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap mmap, const MvxArgs p) {
-  constexpr int kV = stage_values(NT), kCB = stage_bytes(FMT, kV), kWB = w_bytes(FMT, FORM, kV);
+  constexpr int kV = stage_values(RG, NT), kCB = stage_bytes(FMT, kV), kWB = w_bytes(FMT, FORM, RG, kV);
   constexpr int kXB = x_bytes(FORM, NT, kV), kWSlot = slot_of(kCB), kT = 8 * NT;
   constexpr int kXSlot = slot_of(kV), kMetaSlot = slot_of(kV / 4);   // row form
-  constexpr int kBoxRows = PAIR ? kRows / 2 : kRows, kPitch = kBoxRows * 128;
-  constexpr int kOut = PAIR ? kRows / 2 : kRows;   // outputs of a tile
+  constexpr int kOutG = PAIR ? kRows / 2 : kRows, kOut = RG * kOutG;   // outputs of a row group, of a tile
+  constexpr int kPitch = kOut * 128;                                   // a box: kOut rows of one weight
+  constexpr int kRed = red_slices(NT);
   constexpr int kSub = kV / 1024;                  // 128-value parts of a warp's slice
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -518,7 +530,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < kS; ++i) {
       mbar_init(&full[i], 2);   // the weights' bytes and the activations' are announced apart
-      mbar_init(&empty[i], kCWarps);
+      mbar_init(&empty[i], RG * kSlices);   // the warps that read the stage
     }
     fence_mbar_init();
   }
@@ -557,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (FORM != kRowForm) {
             if (lane == 0) {
               const int seg0 = int(b0 >> 7), segs = int((b0 + len + 127) >> 7) - seg0;
-              mbar_expect_tx(&full[s], uint32_t(segs) * kRows * 128);
+              mbar_expect_tx(&full[s], uint32_t(segs) * RG * kRows * 128);
               for (int g = 0; g < segs; ++g) {
                 tma_load_2d(dst + g * kPitch, &wmap, (seg0 + g) * 32, tile * kOut, &full[s]);
                 if (PAIR) tma_load_2d(dst + kWB / 2 + g * kPitch, &w2map, (seg0 + g) * 32, tile * kOut, &full[s]);
@@ -626,7 +638,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // ------------------------------------------------------------------ consumers
   mx_wait();
-  const int ks = warp - 1, g = lane >> 2, t = lane & 3;
+  const int group = (warp - 1) / kSlices, ks = (warp - 1) % kSlices, g = lane >> 2, t = lane & 3;
   const uint32_t sbase = smem_u32(smem), xbase = smem_u32(xres);
   // this thread's activations inside a stage: the codes it loads or supplies the address of (box forms: row lane % 8 and
   // 16-byte chunk lane / 8 of ldmatrix4), and the meta of tokens 8 q + 2 t and 8 q + 2 t + 1. Columns past the call's
@@ -650,8 +662,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   int s = 0;
   uint32_t turn = 0;
   bool live = true;
+  int round = 0;   // tiles so far
   for (int u = blockIdx.x; u < p.units && live; u += gridDim.x) {
-    for (int i = 0; i < p.tiles_per_unit && live; ++i) {
+    for (int i = 0; i < p.tiles_per_unit && live; ++i, ++round) {
       const int tile = u * p.tiles_per_unit + i;
       if (tile >= ntile) break;
       float acc[NT][8];
@@ -662,7 +675,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t low[4];   // row form: low address bits of the four rows' windows
 #pragma unroll
       for (int r = 0; r < 4; ++r) low[r] = FORM == kRowForm ? uint32_t(row_src(tile, 8 * r + g, 0)) : 0u;
+      auto next = [&] {
+        if (++s == kS) {
+          s = 0;
+          turn ^= 1;
+        }
+      };
       for (int st = 0; st < nst; ++st) {
+        if (RG == 1 && ((st + round) & 1) != group) {   // the other group's; swapping the groups swaps two summands
+          next();
+          continue;
+        }
         if (!__all_sync(0xFFFFFFFFu, poll(&full[s], turn))) {
           atomicOr(&g_status, 1u);
           live = false;
@@ -706,28 +729,39 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int r = 0; r < 4; ++r) at.p[r] = sb + (8 * r + g) * kWSlot + ((low[r] + uint32_t(st) * kCB) & 15u);
             slice_dot<FMT, NT, kCols>(at, part, gc, lane, xa, ma, sa, acc);
           } else {
-            const BoxAt<kPitch, PAIR ? kWB / 2 : 16 * 128> at{sb + g * 128, uint32_t(int64_t(st) * kCB) & 127u,
-                                                              uint32_t(g) << 4, sb + (lane & 15) * 128,
+            const uint32_t base = sb + (RG == 2 ? group * kOutG * 128 : 0);
+            const BoxAt<kPitch, PAIR ? kWB / 2 : 16 * 128> at{base + g * 128, uint32_t(int64_t(st) * kCB) & 127u,
+                                                              uint32_t(g) << 4, base + (lane & 15) * 128,
                                                               uint32_t(lane & 7) << 4, uint32_t(lane >> 4) << 4};
             slice_dot<FMT, NT, kCols>(at, part, gc, lane, xa, ma, sa, acc);
           }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[s]);
-        if (++s == kS) {
-          s = 0;
-          turn ^= 1;
-        }
+        next();
       }
-      if (!__all_sync(0xFFFFFFFFu, live)) live = false;
-      // the slices' sums meet: [slice][token][row]
-      asm volatile("bar.sync 1, 256;" ::: "memory");   // the last tile's have been read
+      // the warps' sums meet: [warp][token][row]. Where half of the warps write and the other half adds, the first are
+      // group 1 (one row group) or slices 4 .. 7 of both (two).
+      const bool late = kRed == kCWarps ? false : RG == 1 ? group == 0 : ks < kSlices / 2;
+      const int at = kRed == kCWarps ? group * kSlices + ks : RG == 1 ? ks : group * (kSlices / 2) + ks % (kSlices / 2);
+      float* mine = red + at * kT * kTokStride + 2 * t * kTokStride + g;
+      asm volatile("bar.sync 1, 512;" ::: "memory");   // the last tile's have been read
+      if (!late) {
 #pragma unroll
-      for (int q = 0; q < NT; ++q)
+        for (int q = 0; q < NT; ++q)
 #pragma unroll
-        for (int c = 0; c < 8; ++c)
-          red[(ks * kT + 8 * q + 2 * t + (c & 1)) * kTokStride + 8 * (c >> 1) + g] = acc[q][c];
-      asm volatile("bar.sync 1, 256;" ::: "memory");
+          for (int c = 0; c < 8; ++c) mine[(8 * q + (c & 1)) * kTokStride + 8 * (c >> 1)] = acc[q][c];
+      }
+      asm volatile("bar.sync 1, 512;" ::: "memory");
+      if (kRed != kCWarps) {
+        if (late) {
+#pragma unroll
+          for (int q = 0; q < NT; ++q)
+#pragma unroll
+            for (int c = 0; c < 8; ++c) mine[(8 * q + (c & 1)) * kTokStride + 8 * (c >> 1)] += acc[q][c];
+        }
+        asm volatile("bar.sync 1, 512;" ::: "memory");
+      }
       const int ctid = threadIdx.x - 32;
       for (int o = ctid; o < kT * kOut; o += 32 * kCWarps) {   // whole warps: kOut * 8 is a multiple of 32
         const int tk = o / kOut, r = o % kOut, n = tile * kOut + r;
@@ -736,9 +770,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (in) {
           float a = 0.0f, b = 0.0f;
 #pragma unroll
-          for (int q = 0; q < kSlices; ++q) {
-            a += red[(q * kT + tk) * kTokStride + r];
-            if (PAIR) b += red[(q * kT + tk) * kTokStride + 16 + r];
+          for (int q = 0; q < kRed / 2; ++q) {
+            // one row group: warps q and q + kRed / 2 hold this output's sums; two: the group's own kRed / 2 warps
+            const float* e = red + ((RG == 2 ? r / kOutG * (kRed / 2) : 0) + q) * kT * kTokStride + tk * kTokStride + r % kOutG;
+            constexpr int kOther = kRed / 2 * kT * kTokStride;
+            a += RG == 1 ? e[0] + e[kOther] : e[0];
+            if (PAIR) b += RG == 1 ? e[16] + e[kOther + 16] : e[16];
           }
           if (p.e.bias) a += __ldg(p.e.bias + n);
           if (PAIR && p.e.bias2) b += __ldg(p.e.bias2 + n);
@@ -747,7 +784,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (p.e.y_form != LK_Q8_ROWS) {
           if (in) store_elem(p.e.y, p.e.y_form, int64_t(t0 + tk) * p.n + n, v);
-        } else if (!PAIR) {
+        } else if (kOut % 32 == 0) {
           if (tk < ntok)   // n % 32 == 0: a warp is a whole group of one token
             store_q8(static_cast<uint8_t*>(p.e.y), int64_t(p.tokens) * p.n, int64_t(t0 + tk) * p.n + n, v, lane);
         } else if (i == 0) {
@@ -774,10 +811,10 @@ struct Maps {
   CUtensorMap w, w2, x, m;
 };
 
-template <int FMT, int FORM, bool PAIR, int NT>
+template <int FMT, int FORM, bool PAIR, int NT, int RG>
 int launch(const Maps& m, MvxArgs a, cudaStream_t s) {
-  constexpr int kV = stage_values(NT), kWB = w_bytes(FMT, FORM, kV), kXB = x_bytes(FORM, NT, kV);
-  constexpr int kFixed = 1024 + red_bytes(NT) + kTailBytes;
+  constexpr int kV = stage_values(RG, NT), kWB = w_bytes(FMT, FORM, RG, kV), kXB = x_bytes(FORM, NT, kV);
+  constexpr int kFixed = fixed_bytes(NT);
   static_assert(2 * (kWB + kXB) + kFixed <= kSmemMax, "two stages at least");
   static_assert(2 * kMaxStages * 8 <= 256, "the barriers");
   const int nst = (a.k + kV - 1) / kV;
@@ -786,7 +823,7 @@ int launch(const Maps& m, MvxArgs a, cudaStream_t s) {
   const int room = kSmemMax - kFixed - (a.resident ? nst * kXB : 0), slot = kWB + (a.resident ? 0 : kXB);
   a.stages = room / slot < kMaxStages ? room / slot : kMaxStages;
   const int smem = kFixed + a.stages * slot + (a.resident ? nst * kXB : 0);
-  auto kern = k_mvx<FMT, FORM, PAIR, NT>;
+  auto kern = k_mvx<FMT, FORM, PAIR, NT, RG>;
   static unsigned configured = 0;
   if (!once_per_device(configured)) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
   int dev = 0, sms = 0;
@@ -805,36 +842,53 @@ int launch(const Maps& m, MvxArgs a, cudaStream_t s) {
   return cudaLaunchKernelEx(&cfg, kern, m.w, m.w2, m.x, m.m, a) == cudaSuccess ? LK_OK : LK_ECUDA;
 }
 
+template <int FMT, int FORM, bool PAIR, int NT>
+int launch_r(const Maps& m, const MvxArgs& a, int rg, cudaStream_t s) {
+  if constexpr (two_groups(FMT, FORM, NT)) {
+    if (rg == 2) return launch<FMT, FORM, PAIR, NT, 2>(m, a, s);
+  }
+  return launch<FMT, FORM, PAIR, NT, 1>(m, a, s);
+}
 template <int FMT, int FORM, bool PAIR>
-int launch_t(const Maps& m, const MvxArgs& a, cudaStream_t s) {
-  if (FORM == kBox1 || a.tokens <= 8) return launch<FMT, FORM, PAIR, 1>(m, a, s);
-  if (a.tokens <= 16) return launch<FMT, FORM == kBox1 ? kBox : FORM, PAIR, 2>(m, a, s);
-  return launch<FMT, FORM == kBox1 ? kBox : FORM, PAIR, 4>(m, a, s);
+int launch_t(const Maps& m, const MvxArgs& a, int rg, cudaStream_t s) {
+  if (FORM == kBox1 || a.tokens <= 8) return launch_r<FMT, FORM, PAIR, 1>(m, a, rg, s);
+  if (a.tokens <= 16) return launch_r<FMT, FORM == kBox1 ? kBox : FORM, PAIR, 2>(m, a, rg, s);
+  return launch_r<FMT, FORM == kBox1 ? kBox : FORM, PAIR, 4>(m, a, rg, s);
 }
 
 template <int FMT>
-int launch_f(const MvxArgs& a, cudaStream_t s) {
+int launch_f(MvxArgs a, cudaStream_t s) {
   auto al16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
   const bool pair = a.w2 != nullptr;
   // boxes: rows, codes and meta at 16-byte strides from 16-byte aligned starts
   const bool box = a.rb % 16 == 0 && al16(a.w) && al16(a.w2) && a.k % 64 == 0 && a.k >= 256;
+  const int form = !box ? kRowForm : a.tokens == 1 ? kBox1 : kBox, nt = a.tokens <= 8 ? 1 : a.tokens <= 16 ? 2 : 4;
+  int dev = 0, sms = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int outs = pair ? kRows / 2 : kRows;
+  // 64-row tiles where there are more 32-row ones than SMs
+  const int rg = (a.n + outs - 1) / outs > sms && two_groups(FMT, form, nt) ? 2 : 1;
+  const int tiles = (a.n + rg * outs - 1) / (rg * outs);
+  a.tiles_per_unit = rg == 1 && pair && a.e.y_form == LK_Q8_ROWS ? 2 : 1;   // 32 outputs: a group of the q8 form
+  a.units = (tiles + a.tiles_per_unit - 1) / a.tiles_per_unit;
   Maps m;
   if (!box) {
     memset(&m, 0, sizeof(m));
-    return pair ? launch_t<FMT, kRowForm, true>(m, a, s) : launch_t<FMT, kRowForm, false>(m, a, s);
+    return pair ? launch_t<FMT, kRowForm, true>(m, a, rg, s) : launch_t<FMT, kRowForm, false>(m, a, rg, s);
   }
-  const int rows = pair ? kRows / 2 : kRows, kt = a.tokens <= 8 ? 8 : a.tokens <= 16 ? 16 : 32;
+  const int rows = rg * outs;
   int rc = make_map(&m.w, a.w, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, a.n, a.rb / 4, 32, rows, CU_TENSOR_MAP_SWIZZLE_128B);
   m.w2 = m.x = m.m = m.w;
   if (rc == LK_OK && pair)
     rc = make_map(&m.w2, a.w2, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, a.n, a.rb / 4, 32, rows, CU_TENSOR_MAP_SWIZZLE_128B);
-  if (rc == LK_OK && a.tokens > 1)
-    rc = make_map(&m.x, a.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.tokens, a.k, 128, kt, CU_TENSOR_MAP_SWIZZLE_128B);
-  if (rc == LK_OK && a.tokens > 1)
-    rc = make_map(&m.m, a.meta, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, a.tokens, a.k / 16, 32, kt, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc == LK_OK && form == kBox)
+    rc = make_map(&m.x, a.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.tokens, a.k, 128, 8 * nt, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc == LK_OK && form == kBox)
+    rc = make_map(&m.m, a.meta, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, a.tokens, a.k / 16, 32, 8 * nt, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc != LK_OK) return rc;
-  if (a.tokens == 1) return pair ? launch_t<FMT, kBox1, true>(m, a, s) : launch_t<FMT, kBox1, false>(m, a, s);
-  return pair ? launch_t<FMT, kBox, true>(m, a, s) : launch_t<FMT, kBox, false>(m, a, s);
+  if (form == kBox1) return pair ? launch_t<FMT, kBox1, true>(m, a, rg, s) : launch_t<FMT, kBox1, false>(m, a, rg, s);
+  return pair ? launch_t<FMT, kBox, true>(m, a, rg, s) : launch_t<FMT, kBox, false>(m, a, rg, s);
 }
 
 }  // namespace
@@ -851,9 +905,6 @@ int mv_q8_ex(int fmt, int n, int k, int tokens, const uint8_t* xq, const void* w
   a.w2 = static_cast<const uint8_t*>(w2);
   a.rb = lk_row_bytes(fmt, k);
   a.e = e;
-  const int outs = w2 ? kRows / 2 : kRows, tiles = (n + outs - 1) / outs;
-  a.tiles_per_unit = w2 && e.y_form == LK_Q8_ROWS ? 2 : 1;
-  a.units = (tiles + a.tiles_per_unit - 1) / a.tiles_per_unit;
   if (int64_t(tokens) > 65535 * 32) return LK_ERANGE;
   switch (fmt) {
     case LK_Q4_0: return launch_f<LK_Q4_0>(a, s);

@@ -29,6 +29,8 @@ per-expert output biases (gen_moe.py:958-1007, expert_mv bias=True).
 
 Errors raise LkError (the C ABI's negative return codes). There is no CPU fallback: tensors must be on a CUDA device.
 """
+import functools
+
 import torch
 
 from . import _lib as L
@@ -54,7 +56,8 @@ def _ptr(t):
 
 
 def _stream():
-    return torch.cuda.current_stream().cuda_stream
+    # the handle alone: the Stream object around it costs 3 us, as much as a launch
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _act(act):
@@ -62,7 +65,7 @@ def _act(act):
 
 
 def _f32c(t):
-    return None if t is None else t.contiguous().float()
+    return t if t is None or t.dtype == torch.float32 and t.is_contiguous() else t.contiguous().float()
 
 
 def _cuda(*ts):
@@ -71,9 +74,8 @@ def _cuda(*ts):
             raise L.LkError("liblk ops take CUDA tensors (there is no CPU path)")
 
 
-def _need(ok, what):
-    if not ok:
-        raise L.LkError(what)
+def _fail(what):
+    raise L.LkError(what)
 
 
 def _device(*ts):
@@ -81,13 +83,18 @@ def _device(*ts):
     dev = -1
     for t in ts:
         if t is not None:
-            if not t.is_cuda:
+            d = t.get_device()   # -1 on the CPU
+            if d < 0 or not t.is_cuda:
                 raise L.LkError("liblk ops take CUDA tensors (there is no CPU path)")
-            d = t.get_device()
-            if dev >= 0 and d != dev:
+            if d != dev >= 0:
                 raise L.LkError("the tensors are on different devices")
             dev = d
     return dev
+
+
+@functools.lru_cache(maxsize=None)
+def _weight_row(fid, k):
+    return int(L.load().lk_row_bytes(fid, k))
 
 
 def row_bytes(fmt, k):
@@ -680,39 +687,46 @@ def rms_norm(x, weight, eps=1e-6, residual=None, form="bf16", h=None, y=None):
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return rms_norm(x, weight, eps, residual, form, h, y)
-    _need(form in _NORM_FORMS, f"rms_norm: unknown form {form!r}")
-    _need(x.dim() == 2 and weight.numel() == x.shape[1], "rms_norm: x is [rows][k] and weight [k]")
-    _need(x.dtype in _DT and weight.dtype in _DT, "rms_norm: f32, f16 or bf16 operands")
-    rows, k = x.shape
+    fid = _NORM_FORMS.get(form)
+    if fid is None:
+        _fail(f"rms_norm: unknown form {form!r}")
+    if x.dim() != 2 or weight.numel() != x.shape[1]:
+        _fail("rms_norm: x is [rows][k] and weight [k]")
+    xdt, wdt, rdt = _DT.get(x.dtype), _DT.get(weight.dtype), L.F32
+    if xdt is None or wdt is None:
+        _fail("rms_norm: f32, f16 or bf16 operands")
+    shape = x.shape
+    rows, k = shape
     x = x.contiguous()
     weight = weight.contiguous()
-    rdt = L.F32
     if residual is not None:
-        _need(residual.shape == x.shape and residual.dtype in _DT, "rms_norm: residual is [rows][k], f32, f16 or bf16")
-        rdt = _DT[residual.dtype]
-        if h is None:
-            h = torch.empty_like(residual, memory_format=torch.contiguous_format)
-        _need(h.shape == x.shape and h.dtype == residual.dtype and h.is_contiguous(),
-              "rms_norm: h is contiguous, of the residual's shape and type")
+        rdt = _DT.get(residual.dtype)
+        if rdt is None or residual.shape != shape:
+            _fail("rms_norm: residual is [rows][k], f32, f16 or bf16")
         residual = residual.contiguous()
-    else:
-        _need(h is None, "rms_norm: h without a residual")
-    fid = _NORM_FORMS[form]
+        if h is None:
+            h = torch.empty_like(residual)
+        elif h.shape != shape or h.dtype != residual.dtype or not h.is_contiguous():
+            _fail("rms_norm: h is contiguous, of the residual's shape and type")
+    elif h is not None:
+        _fail("rms_norm: h without a residual")
     scales = None
+    plain = _PLAIN.get(form)
     if y is not None:
-        _need(form in _PLAIN or form == "q8", "rms_norm: y is for the plain and q8 forms")
-        _need(y.is_contiguous() and (y.shape == x.shape and y.dtype == _PLAIN[form] if form in _PLAIN else
-                                     y.dtype == torch.uint8 and y.numel() >= rows * k + rows * (k // 32) * 8),
-              "rms_norm: y does not fit the form")
+        if plain is None and form != "q8":
+            _fail("rms_norm: y is for the plain and q8 forms")
+        if not y.is_contiguous() or (y.dtype != torch.uint8 or y.numel() < rows * k + rows * (k // 32) * 8
+                                     if plain is None else y.shape != shape or y.dtype != plain):
+            _fail("rms_norm: y does not fit the form")
+    elif plain is not None:
+        y = torch.empty(shape, dtype=plain, device=x.device)
     elif form == "q8":
         y = torch.empty(rows * k + rows * (k // 32) * 8, dtype=torch.uint8, device=x.device)
-    elif form in _PLAIN:
-        y = torch.empty(rows, k, dtype=_PLAIN[form], device=x.device)
     else:
-        y = torch.empty(rows, k, dtype=torch.float16 if form == "row_f16" else torch.uint8, device=x.device)
+        y = torch.empty(shape, dtype=torch.float16 if form == "row_f16" else torch.uint8, device=x.device)
         scales = torch.empty(rows, 2, dtype=torch.float32, device=x.device)
-    L.check(L.load().lk_rms_norm(rows, k, _ptr(x), _DT[x.dtype], _ptr(residual), rdt, _ptr(weight),
-                                 _DT[weight.dtype], eps, _ptr(h), fid, _ptr(y), _ptr(scales), _stream()),
+    L.check(L.load().lk_rms_norm(rows, k, _ptr(x), xdt, _ptr(residual), rdt, _ptr(weight), wdt, eps, _ptr(h), fid,
+                                 _ptr(y), _ptr(scales), _stream()),
             "lk_rms_norm")
     out = y if scales is None else (y, scales)
     return out if h is None else (out, h)
@@ -720,34 +734,40 @@ def rms_norm(x, weight, eps=1e-6, residual=None, form="bf16", h=None, y=None):
 
 def _epilogue(name, fmt, w, w2, bias, bias2, act, residual, tokens, n, k, out_dtype, y):
     """What mv_q8_ex and gemm_ex share: the operands checked and made contiguous, the output buffer, the ids."""
-    rb = row_bytes(fmt, k)
-    _need(rb > 0, f"{name}: k is not a whole number of the format's blocks")
+    fid = _fmt(fmt)
+    rb = _weight_row(fid, k)
+    if rb <= 0:
+        _fail(f"{name}: k is not a whole number of the format's blocks")
     for t in (w, w2):
-        _need(t is None or (t.is_contiguous() and t.numel() * t.element_size() >= n * rb),
-              f"{name}: a weight holds fewer than n rows, or is not contiguous")
+        if t is not None and (not t.is_contiguous() or t.numel() * t.element_size() < n * rb):
+            _fail(f"{name}: a weight holds fewer than n rows, or is not contiguous")
     for b in (bias, bias2):
-        _need(b is None or b.numel() == n, f"{name}: a bias holds n values")
+        if b is not None and b.numel() != n:
+            _fail(f"{name}: a bias holds n values")
     act = _act(act if act is not None else "none" if w2 is None else "silu")
     rdt = L.F32
     if residual is not None:
-        _need(residual.shape == (tokens, n) and residual.dtype in _DT,
-              f"{name}: residual is [tokens][n], f32, f16 or bf16")
-        rdt = _DT[residual.dtype]
+        rdt = _DT.get(residual.dtype)
+        if rdt is None or residual.shape != (tokens, n):
+            _fail(f"{name}: residual is [tokens][n], f32, f16 or bf16")
         residual = residual.contiguous()
     if out_dtype == "q8":
         form, size = L.Q8_ROWS, tokens * n + tokens * (n // 32) * 8
-        _need(n % 32 == 0, f"{name}: the q8 output needs n % 32 == 0")
+        if n % 32:
+            _fail(f"{name}: the q8 output needs n % 32 == 0")
         if y is None:
             y = torch.empty(size, dtype=torch.uint8, device=w.device)
-        _need(y.dtype == torch.uint8 and y.is_contiguous() and y.numel() >= size, f"{name}: y is a q8 buffer")
+        elif y.dtype != torch.uint8 or not y.is_contiguous() or y.numel() < size:
+            _fail(f"{name}: y is a q8 buffer")
     else:
-        _need(out_dtype in _DT, f"{name}: out_dtype is f32, f16, bf16 or 'q8'")
-        form = _DT[out_dtype]
+        form = _DT.get(out_dtype)
+        if form is None:
+            _fail(f"{name}: out_dtype is f32, f16, bf16 or 'q8'")
         if y is None:
             y = torch.empty(tokens, n, dtype=out_dtype, device=w.device)
-        _need(y.shape == (tokens, n) and y.dtype == out_dtype and y.is_contiguous(),
-              f"{name}: y is contiguous, [tokens][n] of out_dtype")
-    return _f32c(bias), _f32c(bias2), act, residual, rdt, form, y
+        elif y.shape != (tokens, n) or y.dtype != out_dtype or not y.is_contiguous():
+            _fail(f"{name}: y is contiguous, [tokens][n] of out_dtype")
+    return fid, _f32c(bias), _f32c(bias2), act, residual, rdt, form, y
 
 
 def mv_q8_ex(fmt, w, xq, n, k, tokens, w2=None, bias=None, bias2=None, act=None, residual=None,
@@ -761,11 +781,11 @@ def mv_q8_ex(fmt, w, xq, n, k, tokens, w2=None, bias=None, bias2=None, act=None,
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return mv_q8_ex(fmt, w, xq, n, k, tokens, w2, bias, bias2, act, residual, out_dtype, y, alpha, limit)
-    _need(xq.is_contiguous() and xq.numel() * xq.element_size() >= tokens * k + tokens * (k // 32) * 8,
-          "mv_q8_ex: xq holds fewer than `tokens` rows")
-    bias, bias2, act, residual, rdt, form, y = _epilogue("mv_q8_ex", fmt, w, w2, bias, bias2, act, residual, tokens, n,
-                                                         k, out_dtype, y)
-    L.check(L.load().lk_mv_q8_ex(_fmt(fmt), n, k, tokens, _ptr(xq), _ptr(w), _ptr(w2), _ptr(bias), _ptr(bias2), act,
+    if not xq.is_contiguous() or xq.numel() * xq.element_size() < tokens * k + tokens * (k // 32) * 8:
+        _fail("mv_q8_ex: xq holds fewer than `tokens` rows")
+    fid, bias, bias2, act, residual, rdt, form, y = _epilogue("mv_q8_ex", fmt, w, w2, bias, bias2, act, residual,
+                                                              tokens, n, k, out_dtype, y)
+    L.check(L.load().lk_mv_q8_ex(fid, n, k, tokens, _ptr(xq), _ptr(w), _ptr(w2), _ptr(bias), _ptr(bias2), act,
                                  alpha, limit, _ptr(residual), rdt, _ptr(y), form, _stream()), "lk_mv_q8_ex")
     return y
 
@@ -779,14 +799,16 @@ def gemm_ex(fmt, x16, scales, w, n, w2=None, bias=None, bias2=None, act=None, re
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return gemm_ex(fmt, x16, scales, w, n, w2, bias, bias2, act, residual, out_dtype, y, alpha, limit)
-    _need(x16.dim() == 2 and x16.dtype == torch.float16 and scales.shape == (x16.shape[0], 2)
-          and scales.dtype == torch.float32, "gemm_ex: x16 is [rows][k] f16 and scales [rows][2] f32")
-    _need(out_dtype != "q8", "gemm_ex: out_dtype is f32, f16 or bf16")
+    if (x16.dim() != 2 or x16.dtype != torch.float16 or scales.shape != (x16.shape[0], 2)
+            or scales.dtype != torch.float32):
+        _fail("gemm_ex: x16 is [rows][k] f16 and scales [rows][2] f32")
+    if out_dtype == "q8":
+        _fail("gemm_ex: out_dtype is f32, f16 or bf16")
     rows, k = x16.shape
     x16, scales = x16.contiguous(), scales.contiguous()
-    bias, bias2, act, residual, rdt, form, y = _epilogue("gemm_ex", fmt, w, w2, bias, bias2, act, residual, rows, n, k,
-                                                         out_dtype, y)
-    L.check(L.load().lk_gemm_ex(_fmt(fmt), rows, k, n, _ptr(x16), _ptr(scales), _ptr(w), _ptr(w2), _ptr(bias),
+    fid, bias, bias2, act, residual, rdt, form, y = _epilogue("gemm_ex", fmt, w, w2, bias, bias2, act, residual, rows,
+                                                              n, k, out_dtype, y)
+    L.check(L.load().lk_gemm_ex(fid, rows, k, n, _ptr(x16), _ptr(scales), _ptr(w), _ptr(w2), _ptr(bias),
                                 _ptr(bias2), act, alpha, limit, _ptr(residual), rdt, _ptr(y), form, _stream()),
             "lk_gemm_ex")
     return y

@@ -86,6 +86,13 @@ def test_products(ops, fmt, n, k, tokens):
     check(ops, case(fmt, n, k, tokens, 3))
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("n,k,tokens", [(4809, 256, 1), (4737, 1280, 8), (9500, 512, 3), (4769, 512, 17)])
+def test_more_rows_than_one_tile_per_sm(ops, fmt, n, k, tokens):
+    check(ops, case(fmt, n, k, tokens, 13))
+    check(ops, case(fmt, n // 2 + 1, k, tokens, 14, pair=True, bias=True, res="bf16"), "silu", "bf16")
+
+
 @pytest.mark.parametrize("fmt", ["q4_0", "q8_0", "q5_0", "iq4_nl"])
 @pytest.mark.parametrize("n,k,tokens", [(7, 32, 1), (64, 96, 8), (33, 2880, 5), (20, 1056, 33), (9, 16416, 2)])
 def test_widths_of_single_blocks(ops, fmt, n, k, tokens):
@@ -184,9 +191,11 @@ def test_offsets_past_32_bits(ops):
     for i, r in enumerate(rows.tolist()):
         w[r * rb:(r + 1) * rb] = dev(c["w"][i])
     y = ops.mv_q8_ex("q8_0", w, xq_of(c), n, k, 1)
-    want = run(ops, c)
-    assert torch.equal(y[0, rows.cuda()], want[0])
-    assert int((y != 0).sum()) == int((want != 0).sum())
+    # the split of k follows from n, so the order of the sums does too: each is held to the exact value, not to the other
+    v, ev = ref(c)
+    ok, far = E.within(y[:, rows.cuda()].double().cpu().numpy(), v, ev, "f32")
+    assert ok, far
+    assert int((y != 0).sum()) == int((v != 0).sum())
 
 
 def test_results_repeat_on_other_streams_and_in_graphs(ops):
