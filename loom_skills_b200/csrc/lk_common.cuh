@@ -48,6 +48,17 @@ LK_DEV uint32_t iq4_lookup4(uint32_t idx) {
   return prmt(lo, hi, hsel);
 }
 
+// The 8 nibble codes of a word in bit order -> their codebook bytes, 0..3 in a and 4..7 in b, each XORed with FLIP (0: the
+// biased bytes, 0x80808080: int8). A selector nibble of prmt is a code's low 3 bits, so a masked word selects for four
+// codes in both half-tables, and the codes' top bits choose between the two: 11 instructions for 8 codes.
+template <uint32_t FLIP>
+LK_DEV void iq4_lookup8(uint32_t w, uint32_t& a, uint32_t& b) {
+  const uint32_t s = w & 0x77777777u, m = ((w >> 1) & 0x44444444u) | 0x32103210u;
+  a = prmt(prmt(kIq4Biased0 ^ FLIP, kIq4Biased1 ^ FLIP, s), prmt(kIq4Biased2 ^ FLIP, kIq4Biased3 ^ FLIP, s), m);
+  b = prmt(prmt(kIq4Biased0 ^ FLIP, kIq4Biased1 ^ FLIP, s >> 16), prmt(kIq4Biased2 ^ FLIP, kIq4Biased3 ^ FLIP, s >> 16),
+           m >> 16);
+}
+
 LK_DEV float h2f(uint16_t h) { return __half2float(__ushort_as_half(h)); }
 LK_DEV float bf2f(uint16_t b) { return __uint_as_float(uint32_t(b) << 16); }
 

@@ -340,16 +340,21 @@ struct BoxItem {
       const __half dh = __ushort_as_half(uint16_t(h ? w[0] >> 16 : w[0] & 0xffffu));
       const __half2 scale = __halves2half2(dh, dh);
       const uint32_t off = FMT == LK_Q4_0 ? 0x64086408u : 0x64806480u;   // f16 1024 + 8 | 1024 + 128
+      uint32_t lk[8];   // IQ4_NL: word i's codebook bytes of values 4i, 16 + 4i, 4i + 1, 16 + 4i + 1 | 4i + 2, ...
+      if (FMT == LK_IQ4_NL)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) iq4_lookup8<0>(q[i], lk[2 * i], lk[2 * i + 1]);
 #pragma unroll
       for (int cc = 0; cc < 4; ++cc) {
-        uint32_t t0 = ((cc >= 2) ? (q[2 * (cc & 1)] >> 4) : q[2 * (cc & 1)]) & 0x0F0F0F0Fu;
-        uint32_t t1 = ((cc >= 2) ? (q[2 * (cc & 1) + 1] >> 4) : q[2 * (cc & 1) + 1]) & 0x0F0F0F0Fu;
-        if (FMT == LK_IQ4_NL) {
-          t0 = iq4_lookup4(t0);
-          t1 = iq4_lookup4(t1);
-        }
         uint32_t x[4];
-        magic8(t0, t1, x);
+        if (FMT == LK_IQ4_NL) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = prmt(lk[4 * (cc & 1) + i], 0x64646464u, cc >= 2 ? 0x4341u : 0x4240u);
+        } else {
+          const uint32_t t0 = ((cc >= 2) ? (q[2 * (cc & 1)] >> 4) : q[2 * (cc & 1)]) & 0x0F0F0F0Fu;
+          const uint32_t t1 = ((cc >= 2) ? (q[2 * (cc & 1) + 1] >> 4) : q[2 * (cc & 1) + 1]) & 0x0F0F0F0Fu;
+          magic8(t0, t1, x);
+        }
         uint4 out;
         out.x = hmul2u(hsub2u(x[0], off), scale);
         out.y = hmul2u(hsub2u(x[1], off), scale);

@@ -36,7 +36,11 @@ namespace {
 constexpr int kRows = 32;              // weight rows of a warp
 constexpr int kSlices = 8;             // k slices of a stage, a warp of each group for each
 constexpr int kCWarps = 2 * kSlices;   // consumer warps
-constexpr int kThreads = 32 * (1 + kCWarps);
+// 16 consumer warps and a warpgroup whose first warp is the producer: launched at 96 registers a thread (the most that 640
+// threads can have), of which the producer's 128 threads give 64 each to the consumers' 512 (61440 in all, before and
+// after). The consumers' loop needs about 110: with 96 and a lone producer warp, spills cost 5% (Q4_K) to 30% (Q6_K).
+constexpr int kThreads = 32 * kCWarps + 128, kLaunchRegs = 96, kProducerRegs = 32, kConsumerRegs = 112;
+static_assert(128 * kProducerRegs + 32 * kCWarps * kConsumerRegs <= kThreads * kLaunchRegs, "a split that waits forever");
 constexpr int kTokStride = 36;         // floats between tokens of the partial sums: conflict-free stores
 constexpr int kSmemMax = 227 * 1024;
 constexpr int kMaxStages = 8;
@@ -191,6 +195,8 @@ struct BoxAt {
 template <int FMT>
 struct Slice {
   static constexpr bool kUnsigned = FMT == LK_Q4_K || FMT == LK_Q5_K;
+  // lo and hi hold values 4t, 16 + 4t, 4t + 1, 16 + 4t + 1 and 4t + 2, ...: the activations' words are mixed alike
+  static constexpr bool kMixed = FMT == LK_IQ4_NL || FMT == LK_IQ4_XS;
   static constexpr int kQk = fmt_qk(FMT), kBb = fmt_block_bytes(FMT);
   // byte c of block j, mod 4 (blocks start at a multiple of 8 for j = 0)
   static constexpr int low(int c, int j) { return (j * kBb + c) % 4; }
@@ -259,8 +265,7 @@ struct Slice {
       lo = ((r[j][i] << 4) & kHigh) ^ kTop;
       hi = (r[j][i] & kHigh) ^ kTop;
     } else if constexpr (FMT == LK_IQ4_NL || FMT == LK_IQ4_XS) {
-      lo = iq4_lookup4(r[j][i] & kLow) ^ kTop;
-      hi = iq4_lookup4((r[j][i] >> 4) & kLow) ^ kTop;
+      iq4_lookup8<0x80808080u>(r[j][i], lo, hi);   // values 4t, 16 + 4t, 4t + 1, 16 + 4t + 1 | 4t + 2, ... (kMixed)
     } else if constexpr (FMT == LK_Q8_0) {
       lo = r[2 * j][i];
       hi = r[2 * j + 1][i];
@@ -408,6 +413,24 @@ LK_DEV void store_q8(uint8_t* y, int64_t total, int64_t at, float v, int lane) {
     reinterpret_cast<float2*>(y + total)[at / 32] = make_float2(__half2float(__float2half_rn(d)), float(sum));
 }
 
+// two f32 multiply-adds (multiplications) in one instruction, each rounded as fmaf rounds
+LK_DEV float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 z, x, y, z;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+LK_DEV float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 x, x, y;\n\t"
+      "mov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
 // D += A . B of 16 x 4 by 4 x 8 in tf32 (the low 13 bits of the operands are not read)
 LK_DEV void mma_tf32(float a0, float a1, float b, float (&d)[4]) {
   asm("mma.sync.aligned.m16n8k4.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
@@ -438,10 +461,17 @@ LK_DEV void slice_dot(const At& at, int part, int gc, int lane, const XAt& x, co
         mma_tf32(z[2 * h], z[2 * h + 1], hi, p);
         mma_tf32(z[2 * h], z[2 * h + 1], lo, p);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int c = 0; c < COLS; ++c)
-            acc[q][4 * h + 2 * i + c] = fmaf(-dmin[2 * h + i], p[2 * i + c], acc[q][4 * h + 2 * i + c]);
+        for (int i = 0; i < 2; ++i) {
+          float* a = &acc[q][4 * h + 2 * i];
+          const float dm = -dmin[2 * h + i];
+          if (COLS == 2) {
+            const float2 v = fma2(make_float2(dm, dm), make_float2(p[2 * i], p[2 * i + 1]), make_float2(a[0], a[1]));
+            a[0] = v.x;
+            a[1] = v.y;
+          } else {
+            a[0] = fmaf(dm, p[2 * i], a[0]);
+          }
+        }
       }
     }
   }
@@ -464,6 +494,14 @@ LK_DEV void slice_dot(const At& at, int part, int gc, int lane, const XAt& x, co
     for (int q = 0; q < NT; ++q) {
       uint32_t xw[4];
       x(q, pr, xw);
+      if (Slice<FMT>::kMixed) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t lo8 = xw[2 * k], hi8 = xw[2 * k + 1];
+          xw[2 * k] = prmt(lo8, hi8, 0x5140u);
+          xw[2 * k + 1] = prmt(lo8, hi8, 0x7362u);
+        }
+      }
       uint4 mt[2];
 #pragma unroll
       for (int c = 0; c < COLS; ++c) mt[c] = m(q, c, pr);
@@ -479,6 +517,22 @@ LK_DEV void slice_dot(const At& at, int part, int gc, int lane, const XAt& x, co
           } else {
             mma_k32<Slice<FMT>::kUnsigned>(lo[k][2 * h], lo[k][2 * h + 1], hi[k][2 * h], hi[k][2 * h + 1], xw[2 * k],
                                            xw[2 * k + 1], f);
+          }
+          if (COLS == 2) {   // both columns at once, the same sums as below
+            const float2 d = k ? make_float2(__uint_as_float(mt[0].z), __uint_as_float(mt[1].z))
+                               : make_float2(__uint_as_float(mt[0].x), __uint_as_float(mt[1].x));
+            const float2 off = mul2(make_float2(-kMagic, -kMagic), d);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int r = 2 * h + i;
+              float* p = &acc[q][4 * h + 2 * i];
+              float2 v = make_float2(p[0], p[1]);
+              v = fma2(fma2(make_float2(f[2 * i], f[2 * i + 1]), d, off), make_float2(a[k][r], a[k][r]), v);
+              if (kTwo) v = fma2(fma2(make_float2(e[2 * i], e[2 * i + 1]), d, off), make_float2(b[k][r], b[k][r]), v);
+              p[0] = v.x;
+              p[1] = v.y;
+            }
+            continue;
           }
 #pragma unroll
           for (int c = 0; c < COLS; ++c) {
@@ -544,7 +598,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   const int ntile = (p.n + kOut - 1) / kOut;
 
-  if (warp == 0) {
+  if (warp >= kCWarps) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
+    if (warp != kCWarps) return;
     // ------------------------------------------------------------------ producer
     bool live = true, waited = false, used = false;   // used: the ring has been round once
     int s = 0, round = 0;                              // round: tiles so far
@@ -637,8 +693,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 
   // ------------------------------------------------------------------ consumers
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kConsumerRegs));
   mx_wait();
-  const int group = (warp - 1) / kSlices, ks = (warp - 1) % kSlices, g = lane >> 2, t = lane & 3;
+  const int group = warp / kSlices, ks = warp % kSlices, g = lane >> 2, t = lane & 3;
   const uint32_t sbase = smem_u32(smem), xbase = smem_u32(xres);
   // this thread's activations inside a stage: the codes it loads or supplies the address of (box forms: row lane % 8 and
   // 16-byte chunk lane / 8 of ldmatrix4), and the meta of tokens 8 q + 2 t and 8 q + 2 t + 1. Columns past the call's
@@ -663,8 +720,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t turn = 0;
   bool live = true;
   int round = 0;   // tiles so far
-  for (int u = blockIdx.x; u < p.units && live; u += gridDim.x) {
-    for (int i = 0; i < p.tiles_per_unit && live; ++i, ++round) {
+  // a warp whose wait gave up skips the stages left but comes to every barrier, so that the others end too
+  for (int u = blockIdx.x; u < p.units; u += gridDim.x) {
+    for (int i = 0; i < p.tiles_per_unit; ++i, ++round) {
       const int tile = u * p.tiles_per_unit + i;
       if (tile >= ntile) break;
       float acc[NT][8];
@@ -681,7 +739,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           turn ^= 1;
         }
       };
-      for (int st = 0; st < nst; ++st) {
+      for (int st = 0; st < nst && live; ++st) {
         if (RG == 1 && ((st + round) & 1) != group) {   // the other group's; swapping the groups swaps two summands
           next();
           continue;
@@ -762,7 +820,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         asm volatile("bar.sync 1, 512;" ::: "memory");
       }
-      const int ctid = threadIdx.x - 32;
+      const int ctid = threadIdx.x;
       for (int o = ctid; o < kT * kOut; o += 32 * kCWarps) {   // whole warps: kOut * 8 is a multiple of 32
         const int tk = o / kOut, r = o % kOut, n = tile * kOut + r;
         const bool in = tk < ntok && n < p.n;
@@ -826,6 +884,11 @@ int launch(const Maps& m, MvxArgs a, cudaStream_t s) {
   auto kern = k_mvx<FMT, FORM, PAIR, NT, RG>;
   static unsigned configured = 0;
   if (!once_per_device(configured)) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
+  static const int regs = [&] {
+    cudaFuncAttributes fa;
+    return cudaFuncGetAttributes(&fa, kern) == cudaSuccess ? fa.numRegs : 0;
+  }();
+  if (regs < kLaunchRegs) return LK_ECUDA;   // the consumers' registers would never come free
   int dev = 0, sms = 0;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
