@@ -169,5 +169,6 @@ unsigned int status_mx(bool clear);
 unsigned int status_moeq8(bool clear);
 unsigned int status_gemmx(bool clear);
 unsigned int status_mvx(bool clear);
+unsigned int status_norm(bool clear);
 
 }  // namespace lk

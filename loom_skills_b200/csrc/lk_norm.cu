@@ -80,56 +80,25 @@ struct NormArgs {
   int rows;
 };
 
-// FORM: LK_F32 (any plain type, y_dtype at run time), LK_Q8_ROWS, LK_F16_ROWS or LK_E4M3.
-// VEC: rows of whole 16-byte aligned vectors. Otherwise elements are moved one by one: element u * 8 + j of a thread is
-// t + (8 u + j) T, so a warp still touches consecutive addresses -- except for the q8 form, whose 32-value groups stay
-// in four neighbouring lanes.
-template <int FORM, bool VEC, int NV>
-__global__ void __launch_bounds__(kNormMaxThreads) k_rms_norm(const NormArgs p, int y_dtype) {
-  __shared__ float red[2][32];
-  const int t = threadIdx.x, T = blockDim.x, lane = t & 31, warp = t >> 5, nwarps = T >> 5;
-  const int64_t row = blockIdx.x;
-  const int64_t base = row * p.k;
-  constexpr bool kRuns = VEC || FORM == LK_Q8_ROWS;   // a thread's 8 values are consecutive
-  auto at = [&](int u, int j) { return kRuns ? kVec * (t + u * T) + j : t + (kVec * u + j) * T; };
+// Index in the row of element j of a thread's vector u. VEC: rows of whole 16-byte aligned vectors, t, t + T, ... a
+// thread's. Otherwise elements are moved one by one: t + (8 u + j) T, so a warp still touches consecutive addresses --
+// except for the q8 form, whose 32-value groups stay in four neighbouring lanes.
+template <int FORM, bool VEC>
+LK_DEV int elem_at(int u, int j) {
+  const int t = threadIdx.x, T = blockDim.x;
+  return VEC || FORM == LK_Q8_ROWS ? kVec * (t + u * T) + j : t + (kVec * u + j) * T;
+}
 
-  nm_launch();
-  nm_wait();
-  float v[NV][kVec];
+// From the row's h in registers to its stored output. FORM: LK_F32 (any plain type, y_dtype at run time), LK_Q8_ROWS,
+// LK_F16_ROWS or LK_E4M3. weight(u, w): the weight vector u (VEC); own_row(): runs where every thread of the CTA has its
+// part of the row in registers; red: [2][32].
+template <int FORM, bool VEC, int NV, class Weight, class Own>
+LK_DEV void finish_row(const NormArgs& p, int y_dtype, int64_t row, float (&v)[NV][kVec], float (*red)[32],
+                       const Weight& weight, const Own& own_row) {
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, nwarps = blockDim.x >> 5;
+  const int64_t base = row * p.k;
+  auto at = [](int u, int j) { return elem_at<FORM, VEC>(u, j); };
   float ss = 0.0f;
-#pragma unroll
-  for (int u = 0; u < NV; ++u) {
-    if (VEC) {
-      const bool in = at(u, 0) < p.k;
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) v[u][j] = 0.0f;
-      if (in) load_vec(p.x, p.x_dtype, base + at(u, 0), v[u]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) v[u][j] = at(u, j) < p.k ? load_elem(p.x, p.x_dtype, base + at(u, j)) : 0.0f;
-    }
-  }
-  if (p.res) {
-#pragma unroll
-    for (int u = 0; u < NV; ++u) {
-      if (VEC) {
-        if (at(u, 0) < p.k) {
-          float r[kVec];
-          load_vec(p.res, p.res_dtype, base + at(u, 0), r);
-#pragma unroll
-          for (int j = 0; j < kVec; ++j) v[u][j] += r[j];
-          if (p.h) store_vec(p.h, p.res_dtype, base + at(u, 0), v[u]);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < kVec; ++j)
-          if (at(u, j) < p.k) {
-            v[u][j] += load_elem(p.res, p.res_dtype, base + at(u, j));
-            if (p.h) store_elem(p.h, p.res_dtype, base + at(u, j), v[u][j]);
-          }
-      }
-    }
-  }
 #pragma unroll
   for (int u = 0; u < NV; ++u)
 #pragma unroll
@@ -138,6 +107,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) k_rms_norm(const NormArgs p, 
   for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
   if (lane == 0) red[0][warp] = ss;
   __syncthreads();
+  own_row();
   ss = lane < nwarps ? red[0][lane] : 0.0f;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
@@ -149,7 +119,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) k_rms_norm(const NormArgs p, 
     if (VEC) {
       if (at(u, 0) < p.k) {
         float w[kVec];
-        load_vec(p.weight, p.w_dtype, at(u, 0), w);
+        weight(u, w);
 #pragma unroll
         for (int j = 0; j < kVec; ++j) v[u][j] = v[u][j] * rstd * w[j];
       }
@@ -259,6 +229,148 @@ __global__ void __launch_bounds__(kNormMaxThreads) k_rms_norm(const NormArgs p, 
   }
 }
 
+// A CTA per row.
+template <int FORM, bool VEC, int NV>
+__global__ void __launch_bounds__(kNormMaxThreads) k_rms_norm(const NormArgs p, int y_dtype) {
+  __shared__ float red[2][32];
+  const int64_t base = int64_t(blockIdx.x) * p.k;
+  auto at = [](int u, int j) { return elem_at<FORM, VEC>(u, j); };
+
+  nm_launch();
+  nm_wait();
+  float v[NV][kVec];
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+    if (VEC) {
+      const bool in = at(u, 0) < p.k;
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) v[u][j] = 0.0f;
+      if (in) load_vec(p.x, p.x_dtype, base + at(u, 0), v[u]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) v[u][j] = at(u, j) < p.k ? load_elem(p.x, p.x_dtype, base + at(u, j)) : 0.0f;
+    }
+  }
+  if (p.res) {
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      if (VEC) {
+        if (at(u, 0) < p.k) {
+          float r[kVec];
+          load_vec(p.res, p.res_dtype, base + at(u, 0), r);
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) v[u][j] += r[j];
+          if (p.h) store_vec(p.h, p.res_dtype, base + at(u, 0), v[u]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j)
+          if (at(u, j) < p.k) {
+            v[u][j] += load_elem(p.res, p.res_dtype, base + at(u, j));
+            if (p.h) store_elem(p.h, p.res_dtype, base + at(u, j), v[u][j]);
+          }
+      }
+    }
+  }
+  finish_row<FORM, VEC, NV>(p, y_dtype, blockIdx.x, v, red,
+                            [&](int u, float (&w)[kVec]) { load_vec(p.weight, p.w_dtype, at(u, 0), w); }, [] {});
+}
+
+// Many rows: resident CTAs walk the rows, each with a ring of `slots` rows (x, then the residual) that bulk copies fill
+// while earlier rows are worked on, so HBM is read without a pause; a CTA per row leaves it idle between a row's loads
+// and stores. A slot is free again as soon as the row is in registers, at the barrier of its sum of squares.
+constexpr int kMaxSlots = 4;
+constexpr uint32_t kNormPolls = 1u << 22;
+constexpr int kStreamRows = 256;
+// ring bytes of each of n resident CTAs (the system's 1 KB and the kernel's own arrays aside)
+constexpr int stream_smem(int n) { return 227 * 1024 / n - 2048; }
+template <int NV>
+constexpr int stream_threads() { return NV == 1 ? 128 : NV == 2 ? 512 : 1024; }
+constexpr int kStreamThreadsPerSm = 1024;   // resident at 64 registers
+
+template <int FORM, int NV>
+__global__ void __launch_bounds__(stream_threads<NV>(), kStreamThreadsPerSm / stream_threads<NV>())
+    k_rms_norm_stream(const NormArgs p, int y_dtype, int slots, int slot_bytes) {
+  constexpr bool kHoldW = NV <= 2;   // the weights stay in registers
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ float red[2][32];
+  __shared__ uint64_t full[kMaxSlots];
+  const int t = threadIdx.x;
+  const uint32_t xb = uint32_t(p.k) * (p.x_dtype == LK_F32 ? 4 : 2);
+  const uint32_t rb = p.res ? uint32_t(p.k) * (p.res_dtype == LK_F32 ? 4 : 2) : 0;
+  auto at = [](int u) { return elem_at<FORM, true>(u, 0); };
+  auto fetch = [&](int64_t row, int s) {
+    uint8_t* d = ring + s * slot_bytes;
+    mbar_expect_tx(&full[s], xb + rb);
+    bulk_g2s(d, static_cast<const uint8_t*>(p.x) + row * xb, xb, &full[s]);
+    if (rb) bulk_g2s(d + xb, static_cast<const uint8_t*>(p.res) + row * rb, rb, &full[s]);
+  };
+  nm_launch();
+  if (t == 0) {
+    for (int i = 0; i < slots; ++i) mbar_init(&full[i], 1);
+    fence_mbar_init();
+    nm_wait();
+    for (int i = 0; i < slots; ++i)
+      if (int64_t(blockIdx.x) + int64_t(i) * gridDim.x < p.rows) fetch(int64_t(blockIdx.x) + int64_t(i) * gridDim.x, i);
+  }
+  nm_wait();
+  float wt[kHoldW ? NV : 1][kVec];
+  if (kHoldW)
+#pragma unroll
+    for (int u = 0; u < NV; ++u)
+      if (at(u) < p.k) load_vec(p.weight, p.w_dtype, at(u), wt[u]);
+  __syncthreads();
+  int s = 0;
+  uint32_t phase = 0;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    bool in = false;
+    for (uint32_t q = 0; q < kNormPolls && !in; ++q) in = mbar_try_wait(&full[s], phase);
+    if (!__syncthreads_and(in)) {   // given up: the copies in flight land, then the CTA ends
+      if (t == 0) {
+        atomicOr(&g_status, 1u);
+        for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+      }
+      __syncthreads();
+      return;
+    }
+    const uint8_t* xs = ring + s * slot_bytes;
+    float v[NV][kVec];
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) v[u][j] = 0.0f;
+      if (at(u) < p.k) {
+        load_vec(xs, p.x_dtype, at(u), v[u]);
+        if (p.res) {
+          float r[kVec];
+          load_vec(xs + xb, p.res_dtype, at(u), r);
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) v[u][j] += r[j];
+          if (p.h) store_vec(p.h, p.res_dtype, row * p.k + at(u), v[u]);
+        }
+      }
+    }
+    const int64_t next = row + int64_t(slots) * gridDim.x;
+    finish_row<FORM, true, NV>(
+        p, y_dtype, row, v, red,
+        [&](int u, float (&w)[kVec]) {
+          if (kHoldW) {
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) w[j] = wt[kHoldW ? u : 0][j];
+          } else {
+            load_vec(p.weight, p.w_dtype, at(u), w);
+          }
+        },
+        [&] {
+          if (t == 0 && next < p.rows) fetch(next, s);
+        });
+    if (++s == slots) {
+      s = 0;
+      phase ^= 1;
+    }
+  }
+}
+
 template <int FORM, bool VEC, int NV>
 int launch(const NormArgs& a, int y_dtype, int threads, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
@@ -273,9 +385,42 @@ int launch(const NormArgs& a, int y_dtype, int threads, cudaStream_t s) {
   return cudaLaunchKernelEx(&cfg, k_rms_norm<FORM, VEC, NV>, a, y_dtype) == cudaSuccess ? LK_OK : LK_ECUDA;
 }
 
+template <int FORM, int NV>
+int launch_stream(const NormArgs& a, int y_dtype, int threads, cudaStream_t s) {
+  int dev = 0, sms = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int slot = a.k * ((a.x_dtype == LK_F32 ? 4 : 2) + (!a.res ? 0 : a.res_dtype == LK_F32 ? 4 : 2));
+  int per_sm = kStreamThreadsPerSm / threads;
+  while (per_sm > 1 && stream_smem(per_sm) < 2 * slot) --per_sm;
+  int slots = stream_smem(per_sm) / slot;
+  slots = slots < kMaxSlots ? slots : kMaxSlots;
+  auto kern = k_rms_norm_stream<FORM, NV>;
+  static unsigned configured = 0;
+  if (!once_per_device(configured)) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, stream_smem(1));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.rows < sms * per_sm ? a.rows : sms * per_sm, 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = slots * slot;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, a, y_dtype, slots, slot) == cudaSuccess ? LK_OK : LK_ECUDA;
+}
+
 template <int FORM, bool VEC>
 int pick(const NormArgs& a, int y_dtype, cudaStream_t s) {
   const int nvec = (a.k + kVec - 1) / kVec;
+  const int slot = a.k * ((a.x_dtype == LK_F32 ? 4 : 2) + (!a.res ? 0 : a.res_dtype == LK_F32 ? 4 : 2));
+  if (VEC && a.rows >= kStreamRows && slot <= stream_smem(1)) {
+    const int nv = nvec <= 128 ? 1 : nvec <= 1024 ? 2 : 4, threads = ((nvec + nv - 1) / nv + 31) / 32 * 32;
+    if (nv == 1) return launch_stream<FORM, 1>(a, y_dtype, threads, s);
+    if (nv == 2) return launch_stream<FORM, 2>(a, y_dtype, threads, s);
+    return launch_stream<FORM, 4>(a, y_dtype, threads, s);
+  }
   const int nv = nvec <= kNormMaxThreads ? 1 : nvec <= 2 * kNormMaxThreads ? 2 : 4;
   const int threads = ((nvec + nv - 1) / nv + 31) / 32 * 32;
   if (nv == 1) return launch<FORM, VEC, 1>(a, y_dtype, threads, s);
@@ -300,5 +445,7 @@ int rms_norm(int rows, int k, const void* x, int x_dtype, const void* res, int r
   }
   return vec ? pick<LK_F32, true>(a, form, s) : pick<LK_F32, false>(a, form, s);
 }
+
+LK_STATUS_READER(status_norm)
 
 }  // namespace lk

@@ -32,7 +32,9 @@ def f64(t):
 
 
 SIZES = [(1, 1), (3, 7), (2, 32), (1, 4096), (5, 100), (17, 2880), (257, 256), (3, 8200), (2, 16384), (1, 32768),
-         (2, 20001), (4, 8192), (3, 4100)]
+         (2, 20001), (4, 8192), (3, 4100),
+         # many rows (the kernel that walks them), from several rings an SM to one row a ring
+         (5000, 64), (1500, 256), (9000, 8), (900, 2048), (700, 4096), (601, 5120), (400, 16384), (300, 32768)]
 
 
 @pytest.mark.parametrize("rows,k", SIZES)
