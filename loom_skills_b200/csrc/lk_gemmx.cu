@@ -48,6 +48,7 @@ struct GxArgs {
   int band;        // token tiles walked together (see tile_of)
   int cpr;         // packed chunks (256 values) per k range
   int splits;      // CG = 1: CTAs per cluster
+  int boxed;       // window form: the windows of a stage come in one TMA box (two of a pair)
   Epilogue e;
 };
 
@@ -490,7 +491,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 2) {
     // ------------------------------------------------------------------ packed weights
-    if (lane == 0 && !WIN) {
+    if (lane == 0 && (!WIN || p.boxed)) {
       prefetch_tensormap(&wmap);
       if (PAIR) prefetch_tensormap(&w2map);
     }
@@ -504,7 +505,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!live) break;
         uint8_t* dst = sR + at.s * kRaw;
         uint64_t* bar = &full_r[at.s];
-        if (WIN) {
+        if (WIN && p.boxed) {
+          // every row's window starts at the same byte of its row: a box kRW wide from there
+          if (lane == 0) {
+            const int x = int(int64_t(ks >> 2) * kCB & ~int64_t(15)) / 4;
+            mbar_expect_tx(bar, kRaw);
+            tma_load_2d(dst, &wmap, x, n0, bar);
+            if (PAIR) tma_load_2d(dst + kRaw / 2, &w2map, x, n0, bar);
+          }
+        } else if (WIN) {
           // each lane copies the 16-byte aligned window around its rows' chunk; the stage's bytes are announced first
           uint32_t total = 0;
 #pragma unroll
@@ -586,8 +595,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------------ weight staging
     const int group = (warp - 4) >> 3, dt = (threadIdx.x - 128) & 255;
     const int r = dt >> 1, h = dt & 1;   // tile row, which 32 of the stage's 64 values
-    // where the row's packed chunk sits in a raw stage: box form of a pair, gate rows then up rows
-    const int slot = !WIN && PAIR ? (r & 1) * (kRows / 2) + (r >> 1) : r;
+    // where the row's packed chunk sits in a raw stage: boxes of a pair, gate rows then up rows
+    const int slot = PAIR && (!WIN || p.boxed) ? (r & 1) * (kRows / 2) + (r >> 1) : r;
     Place<kS> at;   // the chunk's first stage
     Place<kR> ar;
     int used = 0;   // stages before the chunk's: the first use of a stage waits for nothing
@@ -835,19 +844,21 @@ int gemm_ex(int fmt, int rows, int k, int n, const uint16_t* x16, const float* s
   a.splits = pl.splits;
   a.cpr = (kchunks + pl.splits - 1) / pl.splits;
   a.e = e;
-  // the Q4 family's 144-byte chunks in 16-byte aligned rows come by TMA boxes, everything else by row windows
-  const bool win = !((fmt == LK_Q4_0 || fmt == LK_Q4_K || fmt == LK_IQ4_NL) && k % 256 == 0 &&
-                     (reinterpret_cast<uintptr_t>(w) & 15) == 0 && (reinterpret_cast<uintptr_t>(w2) & 15) == 0);
+  // Rows at 16-byte strides come by TMA boxes: the Q4 family's 144-byte chunks as they are, of other chunks the window
+  // around them (a copy takes the SM about 85 clocks whatever its size: one box instead of 128 row copies took 200 x 4096 x
+  // 4100 Q6_K from WIN_A to WIN_B us). Anything else: row by row.
+  const bool aligned = a.rb % 16 == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0 && (reinterpret_cast<uintptr_t>(w2) & 15) == 0;
+  const bool win = !((fmt == LK_Q4_0 || fmt == LK_Q4_K || fmt == LK_IQ4_NL) && k % 256 == 0 && aligned);
+  a.boxed = win && aligned;
   CUtensorMap m[3];
   int rc = make_map(&m[0], x16, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, rows, k, kStageK, pl.nt / pl.cg,
                     CU_TENSOR_MAP_SWIZZLE_128B);
-  m[1] = m[2] = m[0];   // the window form reads none
-  if (rc == LK_OK && !win)
-    rc = make_map(&m[1], w, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, n, a.rb / 4, kChunkBytes / 4, outs,
-                  CU_TENSOR_MAP_SWIZZLE_NONE);
-  if (rc == LK_OK && !win && pair)
-    rc = make_map(&m[2], w2, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, n, a.rb / 4, kChunkBytes / 4, outs,
-                  CU_TENSOR_MAP_SWIZZLE_NONE);
+  m[1] = m[2] = m[0];   // row by row: none is read
+  const int box = row_slot_bytes(fmt, win) / 4;
+  if (rc == LK_OK && aligned)
+    rc = make_map(&m[1], w, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, n, a.rb / 4, box, outs, CU_TENSOR_MAP_SWIZZLE_NONE);
+  if (rc == LK_OK && aligned && pair)
+    rc = make_map(&m[2], w2, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, n, a.rb / 4, box, outs, CU_TENSOR_MAP_SWIZZLE_NONE);
   if (rc != LK_OK) return rc;
   if (!win) {
     switch (fmt) {
