@@ -77,9 +77,9 @@ constexpr Rings rings_of(int fmt, bool win, int cg, int nt) {
   }
   return g;
 }
-// the partial tile of a split [NT][128] f32 reuses the rings
+// the partial sums of a split reuse the rings: splits x ceil(nt / 8 / splits) groups of 8 tokens, at most 7 more than nt / 8
 constexpr int body_bytes(int fmt, bool win, int cg, int nt) {
-  const int ring = rings_of(fmt, win, cg, nt).bytes(), part = cg == 1 ? nt * kRows * 4 : 0;
+  const int ring = rings_of(fmt, win, cg, nt).bytes(), part = cg == 1 ? (nt + 56) * kRows * 4 : 0;
   return ring > part ? ring : part;
 }
 
@@ -111,10 +111,9 @@ LK_DEV bool elect_one() {
 LK_DEV void arrive_at(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-LK_DEV float ld_peer(uint32_t cluster_addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
-  return v;
+LK_DEV void st_peer(uint32_t cluster_addr, float x, float y, float z, float w) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_addr), "f"(x), "f"(y), "f"(z), "f"(w)
+               : "memory");
 }
 // Bounded wait
 LK_DEV bool wait_bar(uint64_t* bar, uint32_t phase) {
@@ -622,18 +621,23 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (sub < subs) {
             const bool two = sub + 1 < subs;
             const Place<kS> st = at.ahead(sub), su = at.ahead(sub + 1);
-            if (used + sub >= kS) wait_for(&empty[st.s], st.turn ^ 1, live);
-            if (two && used + sub + 1 >= kS) wait_for(&empty[su.s], su.turn ^ 1, live);
-            if (!live) break;
             uint8_t* d0 = sA + st.s * kABytes;
             uint8_t* d1 = sA + su.s * kABytes;
+            // the MMAs end in order: the later stage being free says that the earlier one is
+            auto stages_free = [&] {
+              if (two && used + sub + 1 >= kS) wait_for(&empty[su.s], su.turn ^ 1, live);
+              else if (used + sub >= kS) wait_for(&empty[st.s], st.turn ^ 1, live);
+              return live;
+            };
             if (WIN) {
+              if (!stages_free()) break;
               dequant_group_win<FMT>(chunk, 2 * sub + h, d0, r, 4 * h);
               if (two) dequant_group_win<FMT>(chunk, 2 * sub + 2 + h, d1, r, 4 * h);
             } else {   // whole chunks only: always two
               BoxItem<FMT> i0, i1;
               i0.load(chunk, sub, h);
               i1.load(chunk, sub + 1, h);
+              if (!stages_free()) break;
               i0.store(d0, r, h, sub);
               i1.store(d1, r, h, sub + 1);
             }
@@ -701,48 +705,55 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncwarp();
 
   if (CG == 1 && p.splits > 1) {
-    // the partial tiles of the k ranges meet: every CTA puts its own in shared memory (the rings are idle: all its MMAs
-    // are done), then finishes every splits-th group of 8 tokens from all of them in range order
-    float* part = reinterpret_cast<float*>(smem);   // [NT][128]
+    // The partial tiles of the k ranges meet. Groups of 8 tokens are dealt to the CTAs in turn; every CTA stores its sums
+    // of a group straight from TMEM into the shared memory of the group's owner (the rings: idle once all MMAs of the
+    // cluster are done, hence the first barrier), which adds them in range order and finishes. Stores of 16 bytes that
+    // nobody waits for: reading the peers' tiles took 7000 clocks of a 200 x 4096 x 4100 call, this PUSH_CLK.
+    uint8_t* part = smem;   // [range][own group][half][128 rows][4 tokens] f32
     int t0, n0;
     tile_of(cluster, t0, n0);
-    if (warp >= kEp0) {
-      const int q = warp & 3;
-      wait_for(&acc_full[0], 0, live);
-      tc_fence_after();
-#pragma unroll 1
-      for (int c = 0; c < NT && t0 + c < p.rows; c += 16) {
-        float v[16];
-        tmem_ld(tmem + c + (uint32_t(32 * q) << 16), v);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) part[(c + i) * kRows + 32 * q + lane] = v[i];
-      }
-      for (int i = threadIdx.x - 32 * kEp0; i < NT; i += 32 * kEpW)
-        stok[i] = t0 + i < p.rows ? __ldg(p.scales + 2 * int64_t(t0 + i) + 1) : 0.0f;
-    }
+    constexpr int kGroups = kThreads / 128;   // all warps take part: a quarter of the lanes each, as TMEM is read
+    const int q = warp & 3, row = 32 * q + lane, own = (NT / 8 + p.splits - 1) / p.splits;
+    wait_for(&acc_full[0], 0, live);
+    tc_fence_after();
+    for (int i = threadIdx.x; i < NT; i += kThreads)
+      stok[i] = t0 + i < p.rows ? __ldg(p.scales + 2 * int64_t(t0 + i) + 1) : 0.0f;
     __syncwarp();
     cluster_barrier();
-    {
-      const int q = warp & 3, row = 32 * q + lane;
-      constexpr int kGroups = kThreads / 128;
 #pragma unroll 1
-      for (int c = 8 * (rank + p.splits * (warp >> 2)); c < NT && t0 + c < p.rows; c += 8 * p.splits * kGroups) {
-        float v[8];
+    for (int c = 16 * (warp >> 2); c < NT && t0 + c < p.rows; c += 16 * kGroups) {
+      float v[16];
+      tmem_ld(tmem + c + (uint32_t(32 * q) << 16), v);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-        for (int s = 0; s < p.splits; ++s) {
-          const uint32_t a = peer_addr(part + c * kRows + row, uint32_t(s));
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] += ld_peer(a + i * kRows * 4);
-        }
-        finish<PAIR, 8>(p, v, stok + c, t0 + c, n0, row);
+      for (int h = 0; h < 2; ++h) {
+        const int g = (c >> 3) + h;
+        const uint32_t a = peer_addr(part, uint32_t(g % p.splits)) + (int(rank) * own + g / p.splits) * 4096 + row * 16;
+        st_peer(a, v[8 * h], v[8 * h + 1], v[8 * h + 2], v[8 * h + 3]);
+        st_peer(a + 2048, v[8 * h + 4], v[8 * h + 5], v[8 * h + 6], v[8 * h + 7]);
       }
+    }
+    __syncwarp();
+    cluster_barrier();   // the last word between the CTAs
+#pragma unroll 1
+    for (int l = warp >> 2; l < own; l += kGroups) {
+      const int c = 8 * (int(rank) + p.splits * l);
+      if (c >= NT || t0 + c >= p.rows) break;
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+      for (int s = 0; s < p.splits; ++s) {
+        const float4* f = reinterpret_cast<const float4*>(part + (s * own + l) * 4096) + row;
+        const float4 x = f[0], y = f[128];
+        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+        v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+      }
+      finish<PAIR, 8>(p, v, stok + c, t0 + c, n0, row);
     }
     __syncwarp();
   }
-  // nobody leaves while a peer may still read its shared memory or signal its barriers
+  // nobody of a pair leaves while the other may still signal its barriers
   tc_fence_before();
-  if (CG == 2 || p.splits > 1) cluster_barrier();
+  if (CG == 2) cluster_barrier();
   else __syncthreads();
   tc_fence_after();
   if (warp == 1) tfree<CG>(tmem, kCols);
