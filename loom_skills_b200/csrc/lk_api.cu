@@ -74,7 +74,7 @@ int64_t lk_row_bytes(int fmt, int64_t k) {
 unsigned int lk_device_status(int clear) {
   return status_mv(clear != 0) | status_gemm(clear != 0) | status_mx(clear != 0) | status_q8(clear != 0) |
          status_moeq8(clear != 0) | status_gemmx(clear != 0) | status_mvx(clear != 0) |
-         status_norm(clear != 0);
+         status_norm(clear != 0) | status_mv1(clear != 0);
 }
 
 int lk_quant_q8(int rows, int k, const void* x, int x_dtype, uint8_t* xq, lk_stream_t stream) {

@@ -73,4 +73,19 @@ struct Epilogue {
   int y_form;
 };
 
+// k_quant_q8's codes and meta of one 32-value group, one value a lane
+LK_DEV void store_q8(uint8_t* y, int64_t total, int64_t at, float v, int lane) {
+  float amax = fabsf(v);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
+  const float d = amax / 127.0f;
+  const int q = amax > 0.0f ? int8_t(int(roundf(v / d))) : 0;
+  reinterpret_cast<int8_t*>(y)[at] = int8_t(q);
+  int sum = q;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+  if (lane == 0)
+    reinterpret_cast<float2*>(y + total)[at / 32] = make_float2(__half2float(__float2half_rn(d)), float(sum));
+}
+
 }  // namespace lk

@@ -708,7 +708,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // The partial tiles of the k ranges meet. Groups of 8 tokens are dealt to the CTAs in turn; every CTA stores its sums
     // of a group straight from TMEM into the shared memory of the group's owner (the rings: idle once all MMAs of the
     // cluster are done, hence the first barrier), which adds them in range order and finishes. Stores of 16 bytes that
-    // nobody waits for: reading the peers' tiles took 7000 clocks of a 200 x 4096 x 4100 call, this PUSH_CLK.
+    // nobody waits for: reading the peers' tiles took 7000 clocks of a 200 x 4096 x 4100 call, pushing them 1400 and
+    // the wait for the stores about 3000.
     uint8_t* part = smem;   // [range][own group][half][128 rows][4 tokens] f32
     int t0, n0;
     tile_of(cluster, t0, n0);
@@ -856,8 +857,8 @@ int gemm_ex(int fmt, int rows, int k, int n, const uint16_t* x16, const float* s
   a.cpr = (kchunks + pl.splits - 1) / pl.splits;
   a.e = e;
   // Rows at 16-byte strides come by TMA boxes: the Q4 family's 144-byte chunks as they are, of other chunks the window
-  // around them (a copy takes the SM about 85 clocks whatever its size: one box instead of 128 row copies took 200 x 4096 x
-  // 4100 Q6_K from WIN_A to WIN_B us). Anything else: row by row.
+  // around them (a copy takes the SM about 85 clocks whatever its size: one box instead of 128 row copies took 2048 x
+  // 4096 x 2 12288 Q6_K from 409 to 401 us). Anything else: row by row.
   const bool aligned = a.rb % 16 == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0 && (reinterpret_cast<uintptr_t>(w2) & 15) == 0;
   const bool win = !((fmt == LK_Q4_0 || fmt == LK_Q4_K || fmt == LK_IQ4_NL) && k % 256 == 0 && aligned);
   a.boxed = win && aligned;

@@ -158,6 +158,9 @@ int rms_norm(int rows, int k, const void* x, int x_dtype, const void* res, int r
              int w_dtype, float eps, void* h, int form, void* y, float* scales, cudaStream_t s);
 int mv_q8_ex(int fmt, int n, int k, int tokens, const uint8_t* xq, const void* w, const void* w2, const Epilogue& e,
              cudaStream_t s);
+// its form for one token, and the calls that form takes
+bool mv_q8_one_takes(int fmt, int k, const void* xq, const void* w, const void* w2);
+int mv_q8_one(int fmt, int n, int k, const uint8_t* xq, const void* w, const void* w2, const Epilogue& e, cudaStream_t s);
 int gemm_ex(int fmt, int rows, int k, int n, const uint16_t* x16, const float* scales, const void* w, const void* w2,
             const Epilogue& e, cudaStream_t s);
 
@@ -170,5 +173,6 @@ unsigned int status_moeq8(bool clear);
 unsigned int status_gemmx(bool clear);
 unsigned int status_mvx(bool clear);
 unsigned int status_norm(bool clear);
+unsigned int status_mv1(bool clear);
 
 }  // namespace lk

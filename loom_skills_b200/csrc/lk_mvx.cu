@@ -52,8 +52,6 @@ LK_DEV void mx_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "
 // How a call's operands reach shared memory, and its tokens: kBox1 is the box form of one token, whose codes need no
 // swizzle (all rows read the same words) and come by plain bulk copies.
 enum { kRowForm = 0, kBox = 1, kBox1 = 2 };
-// values of a stage (rg: the row groups of a tile, 1 or 2); the same in every form, so that all sum in the same order
-__host__ __device__ constexpr int stage_values(int rg, int nt) { return rg == 1 && nt == 1 ? 2048 : 1024; }
 // packed bytes of a row's stage; 128-byte segments that can hold them wherever they start
 __host__ __device__ constexpr int stage_bytes(int fmt, int v) { return v / fmt_qk(fmt) * fmt_block_bytes(fmt); }
 __host__ __device__ constexpr int segments(int fmt, int v) {
@@ -75,10 +73,18 @@ constexpr int red_slices(int nt) { return nt <= 2 ? kCWarps : kCWarps / 2; }
 constexpr int red_bytes(int nt) { return red_slices(nt) * 8 * nt * kTokStride * 4; }
 constexpr int kTailBytes = 256 + 16 * 32 * 4;   // barriers; the first tile of a unit of two (q8 output of a pair)
 constexpr int fixed_bytes(int nt) { return 1024 + red_bytes(nt) + kTailBytes; }
+constexpr bool two_stages(int fmt, int form, int rg, int nt, int v) {
+  return 2 * (w_bytes(fmt, form, rg, v) + x_bytes(form, nt, v)) + fixed_bytes(nt) <= kSmemMax;
+}
+// values of a stage: 2048 for up to 8 tokens where two such stages fit (a stage's waits and addresses cost a warp as much as
+// a third of its 128 values' work: 16.9 -> 16.1 us on the Q4_K pair of 4096 -> 12288 at 8 tokens), else 1024. The same in
+// both forms of one row group, so that those sum in the same order.
+constexpr int stage_values(int fmt, int form, int rg, int nt) {
+  return nt == 1 && (rg == 1 || two_stages(fmt, form, rg, nt, 2048)) ? 2048 : 1024;
+}
 // whether two stages of 64-row tiles fit beside the sums
 constexpr bool two_groups(int fmt, int form, int nt) {
-  const int v = stage_values(2, nt);
-  return form != kRowForm && 2 * (w_bytes(fmt, form, 2, v) + x_bytes(form, nt, v)) + fixed_bytes(nt) <= kSmemMax;
+  return form != kRowForm && two_stages(fmt, form, 2, nt, stage_values(fmt, form, 2, nt));
 }
 
 struct MvxArgs {
@@ -398,21 +404,6 @@ LK_DEV void mma_k16(uint32_t a0, uint32_t a1, uint32_t b0, float (&f)[4]) {
   for (int i = 0; i < 4; ++i) f[i] = __int_as_float(c[i]);
 }
 
-// k_quant_q8's codes and meta of one 32-value group, one value a lane
-LK_DEV void store_q8(uint8_t* y, int64_t total, int64_t at, float v, int lane) {
-  float amax = fabsf(v);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
-  const float d = amax / 127.0f;
-  const int q = amax > 0.0f ? int8_t(int(roundf(v / d))) : 0;
-  reinterpret_cast<int8_t*>(y)[at] = int8_t(q);
-  int sum = q;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-  if (lane == 0)
-    reinterpret_cast<float2*>(y + total)[at / 32] = make_float2(__half2float(__float2half_rn(d)), float(sum));
-}
-
 // two f32 multiply-adds (multiplications) in one instruction, each rounded as fmaf rounds
 LK_DEV float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
@@ -563,7 +554,7 @@ template <int FMT, int FORM, bool PAIR, int NT, int RG>
 __global__ void __launch_bounds__(kThreads, 1)
     k_mvx(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap w2map,
           const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap mmap, const MvxArgs p) {
-  constexpr int kV = stage_values(RG, NT), kCB = stage_bytes(FMT, kV), kWB = w_bytes(FMT, FORM, RG, kV);
+  constexpr int kV = stage_values(FMT, FORM, RG, NT), kCB = stage_bytes(FMT, kV), kWB = w_bytes(FMT, FORM, RG, kV);
   constexpr int kXB = x_bytes(FORM, NT, kV), kWSlot = slot_of(kCB), kT = 8 * NT;
   constexpr int kXSlot = slot_of(kV), kMetaSlot = slot_of(kV / 4);   // row form
   constexpr int kOutG = PAIR ? kRows / 2 : kRows, kOut = RG * kOutG;   // outputs of a row group, of a tile
@@ -871,7 +862,7 @@ struct Maps {
 
 template <int FMT, int FORM, bool PAIR, int NT, int RG>
 int launch(const Maps& m, MvxArgs a, cudaStream_t s) {
-  constexpr int kV = stage_values(RG, NT), kWB = w_bytes(FMT, FORM, RG, kV), kXB = x_bytes(FORM, NT, kV);
+  constexpr int kV = stage_values(FMT, FORM, RG, NT), kWB = w_bytes(FMT, FORM, RG, kV), kXB = x_bytes(FORM, NT, kV);
   constexpr int kFixed = fixed_bytes(NT);
   static_assert(2 * (kWB + kXB) + kFixed <= kSmemMax, "two stages at least");
   static_assert(2 * kMaxStages * 8 <= 256, "the barriers");
@@ -969,6 +960,7 @@ int mv_q8_ex(int fmt, int n, int k, int tokens, const uint8_t* xq, const void* w
   a.rb = lk_row_bytes(fmt, k);
   a.e = e;
   if (int64_t(tokens) > 65535 * 32) return LK_ERANGE;
+  if (tokens == 1 && mv_q8_one_takes(fmt, k, xq, w, w2)) return mv_q8_one(fmt, n, k, xq, w, w2, e, s);
   switch (fmt) {
     case LK_Q4_0: return launch_f<LK_Q4_0>(a, s);
     case LK_Q4_K: return launch_f<LK_Q4_K>(a, s);

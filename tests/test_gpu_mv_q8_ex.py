@@ -86,6 +86,19 @@ def test_products(ops, fmt, n, k, tokens):
     check(ops, case(fmt, n, k, tokens, 3))
 
 
+@pytest.mark.parametrize("fmt", ["q4_0", "q4_k"])
+@pytest.mark.parametrize("k", [4096, 8192, 12288, 16384])
+@pytest.mark.parametrize("n", [1, 5, 33, 512, 2400, 4745])
+def test_one_token_of_long_rows(ops, fmt, k, n):
+    check(ops, case(fmt, n, k, 1, 15, bias=True, res="f32"), "gelu")
+    check(ops, case(fmt, n, k, 1, 16, pair=True, bias=True, res="bf16"), "swiglu_oai", "bf16")
+    if n % 32 == 0:
+        one = case(fmt, n, k, 1, 17, pair=True)
+        assert torch.equal(run(ops, one, out="q8"), ops.quant_q8(run(ops, one)))
+        single = case(fmt, n, k, 1, 18)
+        assert torch.equal(run(ops, single, out="q8"), ops.quant_q8(run(ops, single)))
+
+
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("n,k,tokens", [(4809, 256, 1), (4737, 1280, 8), (9500, 512, 3), (4769, 512, 17)])
 def test_more_rows_than_one_tile_per_sm(ops, fmt, n, k, tokens):
