@@ -65,6 +65,12 @@ LK_DEV void store_vec(void* p, int dtype, int64_t off, const float (&v)[kVec]) {
   *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + off) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+LK_DEV float2 pair_of(const float (&v)[kVec], int j) { return make_float2(v[j], v[j + 1]); }
+LK_DEV void set_pair(float (&v)[kVec], int j, float2 x) {
+  v[j] = x.x;
+  v[j + 1] = x.y;
+}
+
 struct NormArgs {
   int k;
   const void* x;
@@ -98,11 +104,12 @@ LK_DEV void finish_row(const NormArgs& p, int y_dtype, int64_t row, float (&v)[N
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, nwarps = blockDim.x >> 5;
   const int64_t base = row * p.k;
   auto at = [](int u, int j) { return elem_at<FORM, VEC>(u, j); };
-  float ss = 0.0f;
+  float2 sq = make_float2(0.0f, 0.0f);
 #pragma unroll
   for (int u = 0; u < NV; ++u)
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) ss = fmaf(v[u][j], v[u][j], ss);
+    for (int j = 0; j < kVec; j += 2) sq = fma2(pair_of(v[u], j), pair_of(v[u], j), sq);
+  float ss = sq.x + sq.y;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
   if (lane == 0) red[0][warp] = ss;
@@ -121,7 +128,8 @@ LK_DEV void finish_row(const NormArgs& p, int y_dtype, int64_t row, float (&v)[N
         float w[kVec];
         weight(u, w);
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) v[u][j] = v[u][j] * rstd * w[j];
+        for (int j = 0; j < kVec; j += 2)
+          set_pair(v[u], j, mul2(mul2(pair_of(v[u], j), make_float2(rstd, rstd)), pair_of(w, j)));
       }
     } else {
 #pragma unroll
@@ -199,7 +207,7 @@ LK_DEV void finish_row(const NormArgs& p, int y_dtype, int64_t row, float (&v)[N
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) v[u][j] *= s;
+      for (int j = 0; j < kVec; j += 2) set_pair(v[u], j, mul2(pair_of(v[u], j), make_float2(s, s)));
       if (FORM == LK_F16_ROWS) {
         if (VEC) {
           if (at(u, 0) < p.k) store_vec(p.y, LK_F16, base + at(u, 0), v[u]);
