@@ -19,6 +19,10 @@
 // the 128-byte swizzle, which puts the 8 rows x 4 words a warp reads at once into 32 banks; the activations stay in
 // shared memory after a CTA's first tile where they leave three stages of weights. Row form (anything else): a bulk copy
 // per row and token into padded slots; a copy costs about 85 clocks whatever its size, which bounds this form.
+//
+// Measured, a Q4_K pair of 4096 -> 12288 (56.6 MB, 8.8 us at the measured copy rate): 16.1 us at 8 tokens (3.5 TB/s), 23.9 at
+// 16, 35.9 at 32; the loads alone 10.9, 13.1 and 15.7. The rest is instruction issue: one scale per 32 values, row and
+// token. One token of the 4-bit formats is lk_mv1.cu's.
 #include <cstring>
 
 #include "lk_common.cuh"

@@ -4,10 +4,14 @@
 //   v = h * rstd * weight,  rstd = 1 / sqrt(mean(h^2) + eps)     (f32, from the unrounded h)
 //   y = v rounded to f32 / f16 / bf16, or the codes lk_quant_q8, lk_row_scale_f16 or lk_row_scale_f8 make of v
 //
-// One CTA per row. Thread t holds the 8-value vectors t, t + T, ... of the row in registers from the first load to the
-// last store, so x and the residual are read once and h and y written once; the only exchanges are the sum of squares
-// (and for the row-scaled forms the row's maximum) through warp shuffles and one shared array. Bound by HBM at many rows
-// and by launch and load latency at few.
+// A CTA works on a row at a time. Thread t holds the 8-value vectors t, t + T, ... of the row in registers from the first
+// load to the last store, so x and the residual are read once and h and y written once; the only exchanges are the sum of
+// squares (and for the row-scaled forms the row's maximum) through warp shuffles and one shared array.
+//
+// Few rows, and rows that are not whole 16-byte vectors: a CTA per row, as many threads as vectors, bound by the launch and
+// one load latency (1 to 8 rows of 4096: 2.5 to 2.7 us). From 256 rows resident CTAs stream them (k_rms_norm_stream): 2048 x
+// 4096 to row-scaled f16 in 15.1 us (4.4 TB/s, 69 % of the measured copy rate) against 17.1 with a CTA per row, 4096 x 5120
+// to row-scaled e4m3 29.8 against 37.1; 8192 x 5120 to bf16 66 us (5.1 TB/s).
 #include "lk_common.cuh"
 #include "lk_epi.cuh"
 #include "lk_internal.h"
@@ -289,7 +293,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) k_rms_norm(const NormArgs p, 
 // and stores. A slot is free again as soon as the row is in registers, at the barrier of its sum of squares.
 constexpr int kMaxSlots = 4;
 constexpr uint32_t kNormPolls = 1u << 22;
-constexpr int kStreamRows = 256;
+constexpr int kStreamRows = 256;   // fewer rows than that leave most rings a row or two
 // ring bytes of each of n resident CTAs (the system's 1 KB and the kernel's own arrays aside)
 constexpr int stream_smem(int n) { return 227 * 1024 / n - 2048; }
 template <int NV>

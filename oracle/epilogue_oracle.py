@@ -50,9 +50,9 @@ def act_pair(act, g, u, alpha=1.702, limit=7.0):
 
 
 # |d act / d g| is at most 1.13 (tanh and erf GELU; SiLU 1.10; with alpha 1.702 1.10 too, its slope being that of
-# SiLU at alpha g). Evaluating it in f32 loses at most 16 half steps of |g|: expf, tanhf and erff are within 2 steps
-# (4 half steps) of their value, an argument's rounding moves exp or tanh by at most 2 half steps of |g| where they are
-# not yet saturated, and there are up to 5 more products and sums.
+# SiLU at alpha g). Evaluating it in f32 loses at most 16 half steps of |g|: exp, tanh, erf and the division are within 2
+# steps (4 half steps) of their value, an argument's rounding moves exp or tanh by at most 2 half steps of |g| where they
+# are not yet saturated, and there are up to 5 more products and sums.
 SLOPE, ACT_REL = 1.13, 16 * EPS32
 
 
