@@ -33,6 +33,7 @@ static int pair_check(int fmt, int64_t k) {
   return LK_OK;
 }
 
+static constexpr int kMaxOutputs = 1 << 30;   // outputs of an epilogue product: tile arithmetic stays in 32 bits
 static bool plain_dtype(int dt) { return dt == LK_F32 || dt == LK_F16 || dt == LK_BF16; }
 static uintptr_t elem_bytes(int dt) { return dt == LK_F32 ? 4 : dt == LK_E4M3 ? 1 : 2; }
 
@@ -632,6 +633,7 @@ int lk_mv_q8_ex(int fmt, int n, int k, int tokens, const uint8_t* xq, const void
   if (n <= 0 || k <= 0 || tokens < 0 || k % fmt_qk(fmt)) return LK_EINVAL;
   if (!plain_dtype(y_form) && y_form != LK_Q8_ROWS) return LK_EINVAL;
   if (y_form == LK_Q8_ROWS && n % 32) return LK_EINVAL;
+  if (n > kMaxOutputs) return LK_ERANGE;
   if (int rc = epilogue_check(w2, bias, bias2, act, residual, r_dtype, y, y_form)) return rc;
   if (tokens == 0) return LK_OK;
   if (!xq || !w || !y) return LK_EINVAL;
@@ -646,6 +648,7 @@ int lk_gemm_ex(int fmt, int rows, int k, int n, const uint16_t* x16, const float
   if (!mv_format(fmt)) return LK_EUNSUPPORTED;
   if (n <= 0 || k <= 0 || rows < 0 || k % 64 || k % fmt_qk(fmt)) return LK_EINVAL;
   if (!plain_dtype(y_dtype)) return LK_EINVAL;
+  if (n > kMaxOutputs) return LK_ERANGE;
   if (int rc = epilogue_check(w2, bias, bias2, act, residual, r_dtype, y, y_dtype)) return rc;
   if (rows == 0) return LK_OK;
   if (!x16 || !scales || !w || !y) return LK_EINVAL;

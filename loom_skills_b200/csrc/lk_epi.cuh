@@ -1,9 +1,24 @@
 // What the epilogue products (lk_mv_q8_ex, lk_gemm_ex) and the fused norm share: element loads and stores of the three
 // value types, and the activations.
 #pragma once
+#include <atomic>
+
 #include "lk_common.cuh"
 
 namespace lk {
+
+// Lets `kern` take `bytes` of dynamic shared memory on the current device; `done` (a bit a device) says where that is set
+// already. The bit follows the setting: a call that races with the first one sets it again instead of launching without.
+template <class Kernel>
+bool allow_smem(Kernel kern, int bytes, std::atomic<unsigned>& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const unsigned bit = 1u << (dev & 31);
+  if (done.load(std::memory_order_acquire) & bit) return true;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  done.fetch_or(bit, std::memory_order_release);
+  return true;
+}
 
 // element i of an array of LK_F32 / LK_F16 / LK_BF16
 LK_DEV float load_elem(const void* p, int dtype, int64_t i) {

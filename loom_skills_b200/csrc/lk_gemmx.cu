@@ -772,8 +772,8 @@ int launch_t(const CUtensorMap* m, const GxArgs& a, int grid, cudaStream_t s) {
   static_assert(smem <= kSmemMax, "the CTA exceeds shared memory");
   static_assert(rings_of(FMT, WIN, CG, NT).s >= 3 && rings_of(FMT, WIN, CG, NT).r >= 2, "the rings");
   auto kern = k_gemmx<FMT, WIN, PAIR, CG, NT>;
-  static unsigned configured = 0;
-  if (!once_per_device(configured)) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<unsigned> allowed{0};
+  if (!allow_smem(kern, smem, allowed)) return LK_ECUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid, 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);

@@ -208,8 +208,8 @@ int launch(Mv1Args a, cudaStream_t s) {
   constexpr int smem = stages_of(S) * 2 * groups_of(S) * S * kRowSlice;
   static_assert(smem + 2048 <= 227 * 1024, "the ring");
   auto kern = k_mv1<FMT, PAIR, S>;
-  static unsigned configured = 0;
-  if (!once_per_device(configured)) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<unsigned> allowed{0};
+  if (!allow_smem(kern, smem, allowed)) return LK_ECUDA;
   int dev = 0, sms = 0;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);

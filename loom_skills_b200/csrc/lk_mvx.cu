@@ -859,8 +859,8 @@ int launch(const Maps& m, MvxArgs a, cudaStream_t s) {
   a.stages = room / slot < kMaxStages ? room / slot : kMaxStages;
   const int smem = kFixed + a.stages * slot + (a.resident ? nst * kXB : 0);
   auto kern = k_mvx<FMT, FORM, PAIR, NT, RG>;
-  static unsigned configured = 0;
-  if (!once_per_device(configured)) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
+  static std::atomic<unsigned> allowed{0};
+  if (!allow_smem(kern, kSmemMax, allowed)) return LK_ECUDA;
   static const int regs = [&] {
     cudaFuncAttributes fa;
     return cudaFuncGetAttributes(&fa, kern) == cudaSuccess ? fa.numRegs : 0;

@@ -408,8 +408,8 @@ int launch_stream(const NormArgs& a, int y_dtype, int threads, cudaStream_t s) {
   int slots = stream_smem(per_sm) / slot;
   slots = slots < kMaxSlots ? slots : kMaxSlots;
   auto kern = k_rms_norm_stream<FORM, NV>;
-  static unsigned configured = 0;
-  if (!once_per_device(configured)) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, stream_smem(1));
+  static std::atomic<unsigned> allowed{0};
+  if (!allow_smem(kern, stream_smem(1), allowed)) return LK_ECUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.rows < sms * per_sm ? a.rows : sms * per_sm, 1, 1);
   cfg.blockDim = dim3(threads, 1, 1);

@@ -815,7 +815,7 @@ def gemm_ex(fmt, x16, scales, w, n, w2=None, bias=None, bias2=None, act=None, re
 
 
 # formats with integer weight codes: the decode products on int8 activations take them
-_Q8_FORMATS = ("q4_0", "q4_k", "q8_0", "q5_0", "q5_k", "q6_k", "iq4_nl", "iq4_xs")
+_Q8_FORMATS = frozenset(L.FMT_IDS[f] for f in ("q4_0", "q4_k", "q8_0", "q5_0", "q5_k", "q6_k", "iq4_nl", "iq4_xs"))
 
 
 def ffn(fmt, x, norm_w, w_gate, w_up, w_down, h, f, residual=None, eps=1e-6, act="silu", b_gate=None, b_up=None,
@@ -832,7 +832,7 @@ def ffn(fmt, x, norm_w, w_gate, w_up, w_down, h, f, residual=None, eps=1e-6, act
     fd = fmt_down or fmt
     stream = x if residual is None else residual
     if prefill is None:
-        prefill = tokens >= 64 or fmt not in _Q8_FORMATS or fd not in _Q8_FORMATS
+        prefill = tokens >= 64 or _fmt(fmt) not in _Q8_FORMATS or _fmt(fd) not in _Q8_FORMATS
     ep = dict(w2=w_up, bias=b_gate, bias2=b_up, act=act, alpha=alpha, limit=limit)
     form = "row_f16" if prefill else "q8"
     v, s = rms_norm(x, norm_w, eps, residual=residual, form=form) if residual is not None else \

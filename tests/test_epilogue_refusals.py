@@ -41,7 +41,7 @@ def test_norm(kw, code):
 
 @pytest.mark.parametrize("call", [mv, gemm])
 @pytest.mark.parametrize("kw,code", [
-    (dict(n=0), EINVAL), (dict(k=0), EINVAL), (dict(k=128), EINVAL), (dict(form=99), EINVAL), (dict(form=L.E4M3), EINVAL),
+    (dict(n=0), EINVAL), (dict(n=2**30 + 32), ERANGE), (dict(k=0), EINVAL), (dict(k=128), EINVAL), (dict(form=99), EINVAL), (dict(form=L.E4M3), EINVAL),
     (dict(act=99), EINVAL), (dict(act=-1), EINVAL), (dict(act=L.ACT_SWIGLU_OAI), EINVAL),   # needs a pair
     (dict(b2=16), EINVAL),                        # bias2 without w2
     (dict(r=R, rd=99), EINVAL), (dict(r=Y, rd=L.BF16), EINVAL),   # in place of another type

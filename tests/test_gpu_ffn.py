@@ -126,3 +126,59 @@ def test_norm_before_the_other_products(ops):
     e8 = torch.randint(118, 124, (n, h // 32), dtype=torch.uint8, device="cuda")
     assert torch.equal(ops.gemm_mxfp4s_f8("store", x8, s8, nib, e8, n),
                        ops.gemm_mxfp4s_f8("store", *ops.row_scale_f8(v), nib, e8, n))
+
+
+FIRST_CALLS = """
+import threading, torch
+from loom_skills_b200 import ops
+torch.manual_seed(0)
+w = torch.randint(0, 255, (512, 144 * 2), dtype=torch.uint8, device="cuda")
+w[:, 0::144] = w[:, 2::144] = 0
+w[:, 1::144] = w[:, 3::144] = 0x2C          # finite f16 scales and minima
+x = torch.randn(300, 512, device="cuda").bfloat16()
+nw = torch.ones(512, device="cuda")
+def layer(t):
+    return ops.ffn("q4_k", x[:t], nw, w, w, w, 512, 512)
+sizes = [1, 8, 40, 300]
+if MODE == "capture":                       # the first launch of every kernel goes into a graph
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = [layer(t) for t in sizes]
+    g.replay()
+else:                                       # ... or comes from four threads at once
+    got = [None] * 16
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got[i] = layer(sizes[i % 4])
+            torch.cuda.current_stream().synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(16)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+torch.cuda.synchronize()
+for i, y in enumerate(got):
+    assert torch.equal(y, layer(sizes[i % 4])) and torch.isfinite(y.float()).all()
+assert ops.device_status() == 0
+print("same")
+"""
+
+
+@pytest.mark.parametrize("mode", ["capture", "threads"])
+def test_first_calls_of_a_process(ops, mode):
+    import os
+    import subprocess
+    import sys
+    r = subprocess.run([sys.executable, "-c", f"MODE = {mode!r}\n" + FIRST_CALLS], capture_output=True, text=True,
+                       cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
+
+
+def test_formats_by_id(ops):
+    c = torch.randint(0, 255, (64, 144), dtype=torch.uint8, device="cuda")
+    c[:, 0] = c[:, 2] = 0
+    c[:, 1] = c[:, 3] = 0x2C
+    w = c.repeat(4, 1)
+    x, nw = torch.randn(3, 256, device="cuda"), torch.ones(256, device="cuda")
+    by_name = ops.ffn("q4_k", x, nw, w, w, w, 256, 256)
+    assert torch.equal(ops.ffn(ops.L.Q4_K, x, nw, w, w, w, 256, 256), by_name)
+    assert torch.equal(ops.ffn("q4_k", x, nw, w, w, w, 256, 256, prefill=False), by_name)
