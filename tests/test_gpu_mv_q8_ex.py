@@ -86,9 +86,10 @@ def test_products(ops, fmt, n, k, tokens):
     check(ops, case(fmt, n, k, tokens, 3))
 
 
-@pytest.mark.parametrize("fmt", ["q4_0", "q4_k", "iq4_nl"])
+@pytest.mark.parametrize("fmt", ["q4_0", "q4_k", "iq4_nl", "q6_k"])
 @pytest.mark.parametrize("n,k", [(1, 4096), (33, 8192), (4745, 4096), (2400, 8192), (512, 12288), (5, 16384), (2400, 16384),
-                                 (512, 256), (4745, 2304), (2400, 5120), (33, 6400), (512, 13824), (1, 16128)])
+                                 (512, 256), (4745, 2304), (2400, 5120), (33, 6400), (512, 13824), (1, 16128),
+                                 (4745, 2048), (64, 6144), (2400, 14336)])
 def test_one_token_of_long_rows(ops, fmt, k, n):
     check(ops, case(fmt, n, k, 1, 15, bias=True, res="f32"), "gelu")
     check(ops, case(fmt, n, k, 1, 16, pair=True, bias=True, res="bf16"), "swiglu_oai", "bf16")
