@@ -202,3 +202,33 @@ def test_captured_replays_and_another_stream(ops):
         a, ha = ops.rms_norm((x * scale), w, residual=r, form="q8")
         b, hb = ops.rms_norm(ha, w, residual=r, form="q8")
         assert torch.equal(out, a) and torch.equal(out2, b) and torch.equal(h, hb)
+
+
+@pytest.mark.parametrize("rows,k", [(600, 2048), (300, 8192)])
+def test_many_rows_in_place(ops, rows, k):
+    """The stream updated in its own buffer and the norm written over x, while later rows are already being fetched."""
+    x, r, w = make(rows, k, "bf16", "f32", "f32", 31)
+    y0, h0 = ops.rms_norm(x, w, 1e-6, residual=r)
+    xs, rs = x.clone(), r.clone()
+    y, h = ops.rms_norm(xs, w, 1e-6, residual=rs, h=rs, y=xs)
+    assert y.data_ptr() == xs.data_ptr() and h.data_ptr() == rs.data_ptr()
+    assert torch.equal(y, y0) and torch.equal(h, h0)
+    xs = x.clone()                            # h over x
+    y, h = ops.rms_norm(xs, w, 1e-6, residual=x * 0.5, h=xs)
+    y0, h0 = ops.rms_norm(x, w, 1e-6, residual=x * 0.5)
+    assert torch.equal(y, y0) and torch.equal(h, h0)
+    # two graphs of one buffer, replayed on two streams one after the other
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = ops.rms_norm(x, w, 1e-6, residual=r)
+        graphs.append((g, out))
+    for g, out in graphs:
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            g.replay()
+        s.synchronize()
+        assert torch.equal(out[0], ops.rms_norm(x, w, 1e-6, residual=r)[0])
+    assert ops.device_status() == 0
