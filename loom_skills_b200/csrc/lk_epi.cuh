@@ -20,15 +20,6 @@ bool allow_smem(Kernel kern, int bytes, std::atomic<unsigned>& done) {
   return true;
 }
 
-// 16 bytes global -> shared (both 16-byte aligned), and this thread's arrival on `bar` when all its copies so far have landed
-LK_DEV void copy16(void* dst, uintptr_t src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-}
-LK_DEV void arrive_copied(uint64_t* bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-LK_DEV void wait_copied() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-
 // element i of an array of LK_F32 / LK_F16 / LK_BF16
 LK_DEV float load_elem(const void* p, int dtype, int64_t i) {
   if (dtype == LK_BF16) return bf2f(static_cast<const uint16_t*>(p)[i]);

@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < kR; ++i) {
-      mbar_init(&full_r[i], WIN && !p.boxed ? 64 : 1);   // row by row: the threads of two warps
+      mbar_init(&full_r[i], 1);
       mbar_init(&empty_r[i], 8 * kDqG);
     }
     for (int i = 0; i < 2; ++i) {
@@ -494,8 +494,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!live)   // let the copies in flight land before the CTA ends
         for (int i = 0; i < 1000; ++i) __nanosleep(1000);
     }
-  } else if (warp == 2 || (warp == 3 && WIN && !p.boxed)) {
-    // ------------------------------------------------------------------ packed weights (row by row: two warps)
+  } else if (warp == 2) {
+    // ------------------------------------------------------------------ packed weights
     if (lane == 0 && (!WIN || p.boxed)) {
       prefetch_tensormap(&wmap);
       if (PAIR) prefetch_tensormap(&w2map);
@@ -519,22 +519,32 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (PAIR) tma_load_2d(dst + kRaw / 2, &w2map, x, n0, bar);
           }
         } else if (WIN) {
-          // half a warp a row: the 16-byte aligned window around its chunk, 16 bytes a lane. Warp 2 takes the first half of
-          // the rows, warp 3 the second; of a pair the half warps take gate and up.
-          const int hw = lane >> 4, r0 = (warp - 2) * (kRows / 2) + hw;
-          const uint32_t len = uint32_t(min(int64_t(kCB), p.rb - int64_t(ks >> 2) * kCB));
-          const uint32_t step = uint32_t(PAIR ? p.rb : 2 * p.rb);
-          const int left = p.n - n0;   // outputs from the tile's first
-          const uintptr_t first = (PAIR && hw ? reinterpret_cast<uintptr_t>(p.w2p) : reinterpret_cast<uintptr_t>(p.wp)) +
-                                  uintptr_t(int64_t(n0 + (PAIR ? r0 >> 1 : r0)) * p.rb + int64_t(ks >> 2) * kCB);
-          for (int i = 0; i < kRows / 4; ++i) {
-            const int r = r0 + 2 * i;
-            if ((PAIR ? r >> 1 : r) >= left) break;
-            const uintptr_t a = first + uintptr_t(i) * step, a0 = a & ~uintptr_t(15);
-            const uint32_t bytes = uint32_t(((a + len + 15) & ~uintptr_t(15)) - a0);
-            for (uint32_t c = 16 * (lane & 15); c < bytes; c += 256) copy16(dst + r * kRW + c, a0 + c);
+          // each lane copies the 16-byte aligned window around its rows' chunk; the stage's bytes are announced first
+          uint32_t total = 0;
+#pragma unroll
+          for (int i = 0; i < kRows / 32; ++i) {
+            uintptr_t src;
+            uint32_t len;
+            bool in;
+            win_src(lane + 32 * i, n0, ks, src, len, in);
+            if (in) total += uint32_t(((src + len + 15) & ~uintptr_t(15)) - (src & ~uintptr_t(15)));
           }
-          arrive_copied(bar);
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
+          if (lane == 0) mbar_expect_tx(bar, total);
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < kRows / 32; ++i) {
+            uintptr_t src;
+            uint32_t len;
+            bool in;
+            const int r = lane + 32 * i;
+            win_src(r, n0, ks, src, len, in);
+            const uintptr_t a0 = src & ~uintptr_t(15);
+            if (in)
+              bulk_g2s(dst + r * kRW, reinterpret_cast<const void*>(a0),
+                       uint32_t(((src + len + 15) & ~uintptr_t(15)) - a0), bar);
+          }
         } else if (lane == 0) {
           mbar_expect_tx(bar, kRaw);
           tma_load_2d(dst, &wmap, (ks >> 2) * (kChunkBytes / 4), n0, bar);
@@ -545,8 +555,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (at.s == 0) first = false;
       }
     }
-    if (WIN && !p.boxed) wait_copied();
-    else if (!live)
+    if (!live)
       for (int i = 0; i < 1000; ++i) __nanosleep(1000);
   } else if (warp == 1 && !lead) {
     // ------------------------------------------------------------------ tells the leader of this CTA's token tiles

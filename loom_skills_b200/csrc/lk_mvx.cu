@@ -17,9 +17,8 @@
 //
 // Two ways into shared memory. Box form (rows, codes and meta at 16-byte strides): TMA boxes of 128 bytes x 32 rows in
 // the 128-byte swizzle, which puts the 8 rows x 4 words a warp reads at once into 32 banks; the activations stay in
-// shared memory after a CTA's first tile where they leave three stages of weights. Row form (anything else): four warps copy
-// the 16-byte aligned windows around the rows' bytes into padded slots, 16 bytes a lane (a bulk copy per row takes about 85
-// clocks whatever its size: ROWF_TXT).
+// shared memory after a CTA's first tile where they leave three stages of weights. Row form (anything else): a bulk copy
+// per row and token into padded slots; a copy costs about 85 clocks whatever its size, which bounds this form.
 //
 // Measured, a Q4_K pair of 4096 -> 12288 (56.6 MB, 8.8 us at the measured copy rate): 16.1 us at 8 tokens (3.5 TB/s), 23.9 at
 // 16, 35.9 at 32; the loads alone 10.9, 13.1 and 15.7. The rest is instruction issue: one scale per 32 values, row and
@@ -44,13 +43,8 @@ constexpr int kCWarps = 2 * kSlices;   // consumer warps
 // 16 consumer warps and a warpgroup whose first warp is the producer: launched at 96 registers a thread (the most that 640
 // threads can have), of which the producer's 128 threads give 64 each to the consumers' 512 (61440 in all, before and
 // after). The consumers' loop needs about 110: with 96 and a lone producer warp, spills cost 5% (Q4_K) to 30% (Q6_K).
-// The row form's four producer warps work with 64, its consumers with 104.
-constexpr int kThreads = 32 * kCWarps + 128, kLaunchRegs = 96;
-constexpr int producer_regs(bool row_form) { return row_form ? 64 : 32; }
-constexpr int consumer_regs(bool row_form) { return row_form ? 104 : 112; }
-static_assert(128 * producer_regs(false) + 32 * kCWarps * consumer_regs(false) <= kThreads * kLaunchRegs &&
-                  128 * producer_regs(true) + 32 * kCWarps * consumer_regs(true) <= kThreads * kLaunchRegs,
-              "a split that waits forever");
+constexpr int kThreads = 32 * kCWarps + 128, kLaunchRegs = 96, kProducerRegs = 32, kConsumerRegs = 112;
+static_assert(128 * kProducerRegs + 32 * kCWarps * kConsumerRegs <= kThreads * kLaunchRegs, "a split that waits forever");
 constexpr int kTokStride = 36;         // floats between tokens of the partial sums: conflict-free stores
 constexpr int kSmemMax = 227 * 1024;
 constexpr int kMaxStages = 8;
@@ -566,8 +560,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int t0 = blockIdx.y * kT, ntok = min(kT, p.tokens - t0);
   if (threadIdx.x == 0) {
     for (int i = 0; i < kS; ++i) {
-      // the weights' bytes and the activations' are announced apart; row form: the four producer warps' threads
-      mbar_init(&full[i], FORM == kRowForm ? 128 : 2);
+      mbar_init(&full[i], 2);   // the weights' bytes and the activations' are announced apart
       mbar_init(&empty[i], RG * kSlices);   // the warps that read the stage
     }
     fence_mbar_init();
@@ -583,10 +576,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int ntile = (p.n + kOut - 1) / kOut;
 
   if (warp >= kCWarps) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(producer_regs(FORM == kRowForm)));
-    if (FORM != kRowForm && warp != kCWarps) return;
-    // ------------------------------------------------------------------ producer (row form: four warps)
-    const int pw = warp - kCWarps;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
+    if (warp != kCWarps) return;
+    // ------------------------------------------------------------------ producer
     bool live = true, waited = false, used = false;   // used: the ring has been round once
     int s = 0, round = 0;                              // round: tiles so far
     uint32_t turn = 0;
@@ -617,11 +609,14 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
           } else {
-            for (int r = pw; r < kRows; r += 4) {
-              const uintptr_t src = row_src(tile, r, st), a0 = src & ~uintptr_t(15);
-              const uint32_t bytes = window(src, len);
-              for (uint32_t c = 16 * lane; c < bytes; c += 512) copy16(dst + r * kWSlot + c, a0 + c);
-            }
+            const uintptr_t src = row_src(tile, lane, st);
+            const uint32_t bytes = window(src, len);
+            uint32_t total = bytes;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
+            if (lane == 0) mbar_expect_tx(&full[s], total);
+            __syncwarp();
+            bulk_g2s(dst + lane * kWSlot, reinterpret_cast<const void*>(src & ~uintptr_t(15)), bytes, &full[s]);
           }
           if (!waited) {   // the weights of the first stage go out before the previous kernel ends; its output after
             mx_wait();
@@ -647,15 +642,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tma_load_2d(xd + kT * kV + g * kT * 128, &mmap, st * (kV / 16) + g * 32, t0, &full[s]);
             }
           } else {
-            for (int tk = pw; tk < ntok; tk += 4) {
-              const int64_t g0 = int64_t(t0 + tk) * groups + st * (kV / 32);
-              const uintptr_t cs = reinterpret_cast<uintptr_t>(p.codes) + g0 * 32, ms = reinterpret_cast<uintptr_t>(p.meta) + g0 * 8;
-              const uint32_t mb = window(ms, gc * 8);
-              for (uint32_t c = 16 * lane; c < uint32_t(gc) * 32; c += 512) copy16(xd + tk * kXSlot + c, cs + c);
-              for (uint32_t c = 16 * lane; c < mb; c += 512)
-                copy16(xd + kT * kXSlot + tk * kMetaSlot + c, (ms & ~uintptr_t(15)) + c);
+            const int64_t g0 = int64_t(t0 + lane) * groups + st * (kV / 32);
+            const uintptr_t cs = reinterpret_cast<uintptr_t>(p.codes) + g0 * 32, ms = reinterpret_cast<uintptr_t>(p.meta) + g0 * 8;
+            const uint32_t mb = window(ms, gc * 8);
+            uint32_t total = lane < ntok ? gc * 32 + mb : 0;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
+            if (lane == 0) mbar_expect_tx(&full[s], total);
+            __syncwarp();
+            if (lane < ntok) {
+              bulk_g2s(xd + lane * kXSlot, reinterpret_cast<const void*>(cs), gc * 32, &full[s]);
+              bulk_g2s(xd + kT * kXSlot + lane * kMetaSlot, reinterpret_cast<const void*>(ms & ~uintptr_t(15)), mb, &full[s]);
             }
-            arrive_copied(&full[s]);
           }
           __syncwarp();
           if (++s == kS) {
@@ -666,14 +664,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-    if (FORM == kRowForm) wait_copied();
-    else if (!live)   // let the copies in flight land before the CTA ends
+    if (!live)   // let the copies in flight land before the CTA ends
       for (int i = 0; i < 1000; ++i) __nanosleep(1000);
     return;
   }
 
   // ------------------------------------------------------------------ consumers
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(consumer_regs(FORM == kRowForm)));
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kConsumerRegs));
   mx_wait();
   const int group = warp / kSlices, ks = warp % kSlices, g = lane >> 2, t = lane & 3;
   const uint32_t sbase = smem_u32(smem), xbase = smem_u32(xres);
