@@ -75,6 +75,18 @@ LK_DEV void set_pair(float (&v)[kVec], int j, float2 x) {
   v[j + 1] = x.y;
 }
 
+// calls f with a value of the element type `dtype` names: the choice is made once for a row, not once an element, whose loads
+// would then wait for one another
+template <class F>
+LK_DEV void with_type(int dtype, const F& f) {
+  if (dtype == LK_BF16) f(__nv_bfloat16());
+  else if (dtype == LK_F16) f(__half());
+  else f(0.0f);
+}
+// one rounding, to nearest even
+template <typename T>
+LK_DEV void put(T* p, float v) { *p = T(v); }
+
 struct NormArgs {
   int k;
   const void* x;
@@ -125,6 +137,15 @@ LK_DEV void finish_row(const NormArgs& p, int y_dtype, int64_t row, float (&v)[N
   const float rstd = 1.0f / sqrtf(ss / float(p.k) + p.eps);
 
   float amax = 0.0f;
+  if (!VEC)
+    with_type(p.w_dtype, [&](auto one) {
+      const auto* w = static_cast<const decltype(one)*>(p.weight);
+#pragma unroll
+      for (int u = 0; u < NV; ++u)
+#pragma unroll
+        for (int j = 0; j < kVec; ++j)
+          if (at(u, j) < p.k) v[u][j] = v[u][j] * rstd * float(w[at(u, j)]);
+    });
 #pragma unroll
   for (int u = 0; u < NV; ++u) {
     if (VEC) {
@@ -135,25 +156,25 @@ LK_DEV void finish_row(const NormArgs& p, int y_dtype, int64_t row, float (&v)[N
         for (int j = 0; j < kVec; j += 2)
           set_pair(v[u], j, mul2(mul2(pair_of(v[u], j), make_float2(rstd, rstd)), pair_of(w, j)));
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < kVec; ++j)
-        if (at(u, j) < p.k) v[u][j] = v[u][j] * rstd * load_elem(p.weight, p.w_dtype, at(u, j));
     }
 #pragma unroll
     for (int j = 0; j < kVec; ++j) amax = fmaxf(amax, fabsf(v[u][j]));
   }
 
   if (FORM == LK_F32) {
+    if (VEC) {
 #pragma unroll
-    for (int u = 0; u < NV; ++u) {
-      if (VEC) {
+      for (int u = 0; u < NV; ++u)
         if (at(u, 0) < p.k) store_vec(p.y, y_dtype, base + at(u, 0), v[u]);
-      } else {
+    } else {
+      with_type(y_dtype, [&](auto one) {
+        auto* y = static_cast<decltype(one)*>(p.y) + base;
 #pragma unroll
-        for (int j = 0; j < kVec; ++j)
-          if (at(u, j) < p.k) store_elem(p.y, y_dtype, base + at(u, j), v[u][j]);
-      }
+        for (int u = 0; u < NV; ++u)
+#pragma unroll
+          for (int j = 0; j < kVec; ++j)
+            if (at(u, j) < p.k) put(y + at(u, j), v[u][j]);
+      });
     }
   } else if (FORM == LK_Q8_ROWS) {
     // k_quant_q8's rounding of each 32-value group, whose values are in four neighbouring lanes
@@ -258,12 +279,35 @@ __global__ void __launch_bounds__(kNormMaxThreads) k_rms_norm(const NormArgs p, 
 #pragma unroll
       for (int j = 0; j < kVec; ++j) v[u][j] = 0.0f;
       if (in) load_vec(p.x, p.x_dtype, base + at(u, 0), v[u]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) v[u][j] = at(u, j) < p.k ? load_elem(p.x, p.x_dtype, base + at(u, j)) : 0.0f;
     }
   }
-  if (p.res) {
+  if (!VEC) {
+    with_type(p.x_dtype, [&](auto one) {
+      const auto* x = static_cast<const decltype(one)*>(p.x) + base;
+#pragma unroll
+      for (int u = 0; u < NV; ++u)
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) v[u][j] = at(u, j) < p.k ? float(x[at(u, j)]) : 0.0f;
+    });
+    if (p.res)
+      with_type(p.res_dtype, [&](auto one) {
+        using T = decltype(one);
+        const T* r = static_cast<const T*>(p.res) + base;
+        T* h = static_cast<T*>(p.h) + base;
+#pragma unroll
+        for (int u = 0; u < NV; ++u)
+#pragma unroll
+          for (int j = 0; j < kVec; ++j)
+            if (at(u, j) < p.k) v[u][j] += float(r[at(u, j)]);
+        if (p.h)
+#pragma unroll
+          for (int u = 0; u < NV; ++u)
+#pragma unroll
+            for (int j = 0; j < kVec; ++j)
+              if (at(u, j) < p.k) put(h + at(u, j), v[u][j]);
+      });
+  }
+  if (VEC && p.res) {
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
       if (VEC) {
@@ -274,13 +318,6 @@ __global__ void __launch_bounds__(kNormMaxThreads) k_rms_norm(const NormArgs p, 
           for (int j = 0; j < kVec; ++j) v[u][j] += r[j];
           if (p.h) store_vec(p.h, p.res_dtype, base + at(u, 0), v[u]);
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < kVec; ++j)
-          if (at(u, j) < p.k) {
-            v[u][j] += load_elem(p.res, p.res_dtype, base + at(u, j));
-            if (p.h) store_elem(p.h, p.res_dtype, base + at(u, j), v[u][j]);
-          }
       }
     }
   }

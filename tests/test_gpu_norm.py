@@ -34,7 +34,9 @@ def f64(t):
 SIZES = [(1, 1), (3, 7), (2, 32), (1, 4096), (5, 100), (17, 2880), (257, 256), (3, 8200), (2, 16384), (1, 32768),
          (2, 20001), (4, 8192), (3, 4100),
          # many rows (the kernel that walks them), from several rings an SM to one row a ring
-         (5000, 64), (1500, 256), (9000, 8), (900, 2048), (700, 4096), (601, 5120), (400, 16384), (300, 32768)]
+         (5000, 64), (1500, 256), (9000, 8), (900, 2048), (700, 4096), (601, 5120), (400, 16384), (300, 32768),
+         # ... of odd widths
+         (700, 4097), (1200, 99), (300, 16001), (900, 356), (2000, 33), (256, 32767)]
 
 
 @pytest.mark.parametrize("rows,k", SIZES)
@@ -204,7 +206,7 @@ def test_captured_replays_and_another_stream(ops):
         assert torch.equal(out, a) and torch.equal(out2, b) and torch.equal(h, hb)
 
 
-@pytest.mark.parametrize("rows,k", [(600, 2048), (300, 8192)])
+@pytest.mark.parametrize("rows,k", [(600, 2048), (300, 8192), (500, 2049), (300, 8190)])
 def test_many_rows_in_place(ops, rows, k):
     """The stream updated in its own buffer and the norm written over x, while later rows are already being fetched."""
     x, r, w = make(rows, k, "bf16", "f32", "f32", 31)
