@@ -34,6 +34,8 @@ namespace lk {
 
 int make_map(CUtensorMap* map, const void* base, CUtensorMapDataType dt, int elem_bytes, int64_t rows, int64_t cols,
              int box_cols, int box_rows, CUtensorMapSwizzle swz);
+int encode_tiled(CUtensorMap* map, CUtensorMapDataType dt, int rank, const void* base, const cuuint64_t* dims,
+                 const cuuint64_t* strides, const cuuint32_t* box, const cuuint32_t* estr, CUtensorMapSwizzle swz);
 
 namespace {
 
@@ -54,8 +56,15 @@ struct GxArgs {
   int band;        // token tiles walked together (see tile_of)
   int cpr;         // packed chunks (256 values) per k range
   int splits;      // CG = 1: CTAs per cluster
-  int boxed;       // window form: the windows of a stage come in one TMA box (two of a pair)
+  int boxed;       // window form: the windows of a stage come in TMA boxes, one of a weight's rows of each phase
+  int lp;          // log2 of the phases (see WeightMaps)
   Epilogue e;
+};
+
+// The packed weights' tensor maps: w, w2 of every phase. A row stride that is no multiple of 16 bytes is one after P = 2, 4
+// or 8 rows: rows of one phase, r = P j + f, are a tensor of their own from the 16-byte boundary at or before row f.
+struct WeightMaps {
+  CUtensorMap w[8], w2[8];
 };
 
 // Staging warps: groups of 8 that take the stages in turn.
@@ -385,8 +394,7 @@ LK_DEV void dequant_group_win(const uint8_t* chunk, int j, uint8_t* tile, int r,
 
 template <int FMT, bool WIN, bool PAIR, int CG, int NT>
 __global__ void __launch_bounds__(kThreads, 1)
-    k_gemmx(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
-            const __grid_constant__ CUtensorMap w2map, const GxArgs p) {
+    k_gemmx(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ WeightMaps wm, const GxArgs p) {
   constexpr Rings kG = rings_of(FMT, WIN, CG, NT);
   constexpr int kB = kG.b_bytes, kRaw = kG.raw_bytes, kS = kG.s, kR = kG.r, kBatch = kS >= 5 ? 2 : 1;
   constexpr int kRW = row_slot_bytes(FMT, WIN);
@@ -497,8 +505,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 2) {
     // ------------------------------------------------------------------ packed weights
     if (lane == 0 && (!WIN || p.boxed)) {
-      prefetch_tensormap(&wmap);
-      if (PAIR) prefetch_tensormap(&w2map);
+      prefetch_tensormap(&wm.w[0]);
+      if (PAIR) prefetch_tensormap(&wm.w2[0]);
     }
     Place<kR> at;
     bool first = true;
@@ -511,12 +519,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint8_t* dst = sR + at.s * kRaw;
         uint64_t* bar = &full_r[at.s];
         if (WIN && p.boxed) {
-          // every row's window starts at the same byte of its row: a box kRW wide from there
+          // the windows of a phase start at the same byte of their rows: a box kRW wide from there
           if (lane == 0) {
-            const int x = int(int64_t(ks >> 2) * kCB & ~int64_t(15)) / 4;
+            const int64_t c0 = int64_t(ks >> 2) * kCB;
             mbar_expect_tx(bar, kRaw);
-            tma_load_2d(dst, &wmap, x, n0, bar);
-            if (PAIR) tma_load_2d(dst + kRaw / 2, &w2map, x, n0, bar);
+            for (int f = 0; f < 1 << p.lp; ++f) {
+              uint8_t* d = dst + f * (kOut >> p.lp) * kRW;
+              const int64_t lead = (reinterpret_cast<uintptr_t>(p.wp) + uintptr_t(f * p.rb)) & 15;
+              tma_load_2d(d, &wm.w[f], int((c0 + lead) & ~int64_t(15)) / 4, n0 >> p.lp, bar);
+              if (PAIR) {
+                const int64_t lead2 = (reinterpret_cast<uintptr_t>(p.w2p) + uintptr_t(f * p.rb)) & 15;
+                tma_load_2d(d + kRaw / 2, &wm.w2[f], int((c0 + lead2) & ~int64_t(15)) / 4, n0 >> p.lp, bar);
+              }
+            }
           }
         } else if (WIN) {
           // each lane copies the 16-byte aligned window around its rows' chunk; the stage's bytes are announced first
@@ -547,8 +562,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         } else if (lane == 0) {
           mbar_expect_tx(bar, kRaw);
-          tma_load_2d(dst, &wmap, (ks >> 2) * (kChunkBytes / 4), n0, bar);
-          if (PAIR) tma_load_2d(dst + kRaw / 2, &w2map, (ks >> 2) * (kChunkBytes / 4), n0, bar);
+          tma_load_2d(dst, &wm.w[0], (ks >> 2) * (kChunkBytes / 4), n0, bar);
+          if (PAIR) tma_load_2d(dst + kRaw / 2, &wm.w2[0], (ks >> 2) * (kChunkBytes / 4), n0, bar);
         }
         __syncwarp();
         at.next();
@@ -600,8 +615,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------------ weight staging
     const int group = (warp - 4) >> 3, dt = (threadIdx.x - 128) & 255;
     const int r = dt >> 1, h = dt & 1;   // tile row, which 32 of the stage's 64 values
-    // where the row's packed chunk sits in a raw stage: boxes of a pair, gate rows then up rows
-    const int slot = PAIR && (!WIN || p.boxed) ? (r & 1) * (kRows / 2) + (r >> 1) : r;
+    // where the row's packed chunk sits in a raw stage: boxes of a pair, gate rows then up rows; of a weight, phase by phase
+    const bool split = PAIR && (!WIN || p.boxed);
+    const int ro = split ? r >> 1 : r, lp = WIN && p.boxed ? p.lp : 0;
+    const int slot = (split ? (r & 1) * (kRows / 2) : 0) + (ro & ((1 << lp) - 1)) * (kOut >> lp) + (ro >> lp);
     Place<kS> at;   // the chunk's first stage
     Place<kR> ar;
     int used = 0;   // stages before the chunk's: the first use of a stage waits for nothing
@@ -767,7 +784,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 template <int FMT, bool WIN, bool PAIR, int CG, int NT>
-int launch_t(const CUtensorMap* m, const GxArgs& a, int grid, cudaStream_t s) {
+int launch_t(const CUtensorMap& xm, const WeightMaps& m, const GxArgs& a, int grid, cudaStream_t s) {
   constexpr int smem = 1024 + body_bytes(FMT, WIN, CG, NT) + kTailBytes;
   static_assert(smem <= kSmemMax, "the CTA exceeds shared memory");
   static_assert(rings_of(FMT, WIN, CG, NT).s >= 3 && rings_of(FMT, WIN, CG, NT).r >= 2, "the rings");
@@ -787,7 +804,7 @@ int launch_t(const CUtensorMap* m, const GxArgs& a, int grid, cudaStream_t s) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, kern, m[0], m[1], m[2], a) == cudaSuccess ? LK_OK : LK_ECUDA;
+  return cudaLaunchKernelEx(&cfg, kern, xm, m, a) == cudaSuccess ? LK_OK : LK_ECUDA;
 }
 
 struct Plan {
@@ -795,10 +812,10 @@ struct Plan {
 };
 
 template <int FMT, bool WIN>
-int launch_f(const Plan& pl, bool pair, const CUtensorMap* m, const GxArgs& a, cudaStream_t s) {
+int launch_f(const Plan& pl, bool pair, const CUtensorMap& xm, const WeightMaps& m, const GxArgs& a, cudaStream_t s) {
 #define LK_GX(CG, NT)                                             \
   if (pl.cg == CG && pl.nt == NT)                                 \
-    return pair ? launch_t<FMT, WIN, true, CG, NT>(m, a, pl.grid, s) : launch_t<FMT, WIN, false, CG, NT>(m, a, pl.grid, s);
+    return pair ? launch_t<FMT, WIN, true, CG, NT>(xm, m, a, pl.grid, s) : launch_t<FMT, WIN, false, CG, NT>(xm, m, a, pl.grid, s);
   LK_GX(2, 256)
   LK_GX(1, 256)
   LK_GX(1, 128)
@@ -862,42 +879,55 @@ int gemm_ex(int fmt, int rows, int k, int n, const uint16_t* x16, const float* s
   a.splits = pl.splits;
   a.cpr = (kchunks + pl.splits - 1) / pl.splits;
   a.e = e;
-  // Rows at 16-byte strides come by TMA boxes: the Q4 family's 144-byte chunks as they are, of other chunks the window
-  // around them (a copy takes the SM about 85 clocks whatever its size: one box instead of 128 row copies took 2048 x
-  // 4096 x 2 12288 Q6_K from 409 to 401 us). Anything else: row by row.
-  const bool aligned = a.rb % 16 == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0 && (reinterpret_cast<uintptr_t>(w2) & 15) == 0;
-  const bool win = !((fmt == LK_Q4_0 || fmt == LK_Q4_K || fmt == LK_IQ4_NL) && k % 256 == 0 && aligned);
-  a.boxed = win && aligned;
-  CUtensorMap m[3];
-  int rc = make_map(&m[0], x16, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, rows, k, kStageK, pl.nt / pl.cg,
+  // Rows come by TMA boxes: the Q4 family's 144-byte chunks as they are, of other chunks the window around them, a box for
+  // each phase of the row stride. A copy takes the SM about 85 clocks whatever its size: 4 boxes instead of 128 row copies
+  // took 430 x 2688 x 20615 Q8_0 from 170 to 75 us, 3201 x 10880 x 947 IQ4_NL from 231 to 103. Row by row: fewer rows than
+  // phases, and strides of 16 bytes from a start that is not a multiple of 16.
+  const bool al16 = (reinterpret_cast<uintptr_t>(w) & 15) == 0 && (reinterpret_cast<uintptr_t>(w2) & 15) == 0;
+  const bool win = !((fmt == LK_Q4_0 || fmt == LK_Q4_K || fmt == LK_IQ4_NL) && k % 256 == 0 && al16);
+  a.lp = a.rb % 16 == 0 ? 0 : a.rb % 8 == 0 ? 1 : a.rb % 4 == 0 ? 2 : 3;
+  const int phases = 1 << a.lp;
+  // (of one phase an aligned start, so that no row reaches into the next one's stride; n rows at least one of each)
+  const bool boxes = a.rb % 2 == 0 && n >= phases && (a.lp > 0 || al16);
+  a.boxed = win && boxes;
+  CUtensorMap xm;
+  int rc = make_map(&xm, x16, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, rows, k, kStageK, pl.nt / pl.cg,
                     CU_TENSOR_MAP_SWIZZLE_128B);
-  m[1] = m[2] = m[0];   // row by row: none is read
-  const int box = row_slot_bytes(fmt, win) / 4;
-  if (rc == LK_OK && aligned)
-    rc = make_map(&m[1], w, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, n, a.rb / 4, box, outs, CU_TENSOR_MAP_SWIZZLE_NONE);
-  if (rc == LK_OK && aligned && pair)
-    rc = make_map(&m[2], w2, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, n, a.rb / 4, box, outs, CU_TENSOR_MAP_SWIZZLE_NONE);
+  WeightMaps m;
+  for (int f = 0; f < 8; ++f) m.w[f] = m.w2[f] = xm;   // row by row: none is read
+  if (boxes)
+    for (int f = 0; f < phases && rc == LK_OK; ++f) {
+      const cuuint32_t box[2] = {cuuint32_t(row_slot_bytes(fmt, win) / 4), cuuint32_t(outs / phases)}, estr[2] = {1, 1};
+      const cuuint64_t strides[1] = {cuuint64_t(a.rb) * phases};
+      for (int q = 0; q < (pair ? 2 : 1) && rc == LK_OK; ++q) {
+        const uintptr_t row = reinterpret_cast<uintptr_t>(q ? w2 : w) + uintptr_t(a.rb) * f;
+        const cuuint64_t dims[2] = {cuuint64_t(((row & 15) + a.rb + 3) / 4), cuuint64_t((n - f + phases - 1) / phases)};
+        rc = encode_tiled(q ? &m.w2[f] : &m.w[f], CU_TENSOR_MAP_DATA_TYPE_UINT32, 2,
+                          reinterpret_cast<const void*>(row & ~uintptr_t(15)), dims, strides, box, estr,
+                          CU_TENSOR_MAP_SWIZZLE_NONE);
+      }
+    }
   if (rc != LK_OK) return rc;
   if (!win) {
     switch (fmt) {
-      case LK_Q4_0: return launch_f<LK_Q4_0, false>(pl, pair, m, a, s);
-      case LK_Q4_K: return launch_f<LK_Q4_K, false>(pl, pair, m, a, s);
-      case LK_IQ4_NL: return launch_f<LK_IQ4_NL, false>(pl, pair, m, a, s);
+      case LK_Q4_0: return launch_f<LK_Q4_0, false>(pl, pair, xm, m, a, s);
+      case LK_Q4_K: return launch_f<LK_Q4_K, false>(pl, pair, xm, m, a, s);
+      case LK_IQ4_NL: return launch_f<LK_IQ4_NL, false>(pl, pair, xm, m, a, s);
     }
     return LK_EUNSUPPORTED;
   }
   switch (fmt) {
-    case LK_Q4_0: return launch_f<LK_Q4_0, true>(pl, pair, m, a, s);
-    case LK_Q4_K: return launch_f<LK_Q4_K, true>(pl, pair, m, a, s);
-    case LK_IQ4_NL: return launch_f<LK_IQ4_NL, true>(pl, pair, m, a, s);
-    case LK_Q5_0: return launch_f<LK_Q5_0, true>(pl, pair, m, a, s);
-    case LK_Q8_0: return launch_f<LK_Q8_0, true>(pl, pair, m, a, s);
-    case LK_Q5_K: return launch_f<LK_Q5_K, true>(pl, pair, m, a, s);
-    case LK_Q6_K: return launch_f<LK_Q6_K, true>(pl, pair, m, a, s);
-    case LK_IQ4_XS: return launch_f<LK_IQ4_XS, true>(pl, pair, m, a, s);
-    case LK_Q3_K: return launch_f<LK_Q3_K, true>(pl, pair, m, a, s);
-    case LK_IQ3_S: return launch_f<LK_IQ3_S, true>(pl, pair, m, a, s);
-    case LK_MXFP4: return launch_f<LK_MXFP4, true>(pl, pair, m, a, s);
+    case LK_Q4_0: return launch_f<LK_Q4_0, true>(pl, pair, xm, m, a, s);
+    case LK_Q4_K: return launch_f<LK_Q4_K, true>(pl, pair, xm, m, a, s);
+    case LK_IQ4_NL: return launch_f<LK_IQ4_NL, true>(pl, pair, xm, m, a, s);
+    case LK_Q5_0: return launch_f<LK_Q5_0, true>(pl, pair, xm, m, a, s);
+    case LK_Q8_0: return launch_f<LK_Q8_0, true>(pl, pair, xm, m, a, s);
+    case LK_Q5_K: return launch_f<LK_Q5_K, true>(pl, pair, xm, m, a, s);
+    case LK_Q6_K: return launch_f<LK_Q6_K, true>(pl, pair, xm, m, a, s);
+    case LK_IQ4_XS: return launch_f<LK_IQ4_XS, true>(pl, pair, xm, m, a, s);
+    case LK_Q3_K: return launch_f<LK_Q3_K, true>(pl, pair, xm, m, a, s);
+    case LK_IQ3_S: return launch_f<LK_IQ3_S, true>(pl, pair, xm, m, a, s);
+    case LK_MXFP4: return launch_f<LK_MXFP4, true>(pl, pair, xm, m, a, s);
   }
   return LK_EUNSUPPORTED;
 }
