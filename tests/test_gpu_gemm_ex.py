@@ -198,3 +198,31 @@ def test_refusals(ops):
         ops.gemm_ex("q4_k", x, sc[:3], w, 64)
     with pytest.raises(ops.L.LkError):
         ops.gemm_ex("q4_k", x[:, :500], sc, w, 64)
+
+
+# row strides of every remainder by 16 bytes: one to eight phases
+STRIDES = [("q4_0", 320), ("q4_0", 640), ("iq4_nl", 704), ("q8_0", 320), ("q8_0", 1152), ("q5_0", 320), ("q6_k", 768),
+           ("q6_k", 512), ("q3_k", 768), ("iq3_s", 512), ("iq4_xs", 768), ("mxfp4", 320), ("mxfp4", 384)]
+
+
+@pytest.mark.parametrize("fmt,k", STRIDES)
+@pytest.mark.parametrize("rows,n", [(40, 3), (33, 131), (300, 700), (600, 9), (257, 2050)])
+def test_row_strides_of_every_phase(ops, fmt, k, rows, n):
+    check(ops, case(fmt, rows, k, n, 41, bias=True, res="f32"), "gelu")
+    check(ops, case(fmt, rows, k, n, 42, pair=True, bias=True), "silu", "bf16")
+
+
+@pytest.mark.parametrize("fmt,k,off", [("q4_0", 320, 2), ("q8_0", 320, 6), ("iq4_nl", 704, 14), ("q6_k", 768, 10),
+                                       ("mxfp4", 320, 3), ("q4_k", 512, 8)])
+def test_weights_off_the_16_byte_boundary(ops, fmt, k, off):
+    c = case(fmt, 70, k, 150, 43, pair=True)
+    want = run(ops, c)
+
+    def moved(a):
+        buf = torch.zeros(a.size + 64, dtype=torch.uint8, device="cuda")
+        buf[off:off + a.size] = dev(a).view(-1)
+        return buf[off:off + a.size]
+
+    y = ops.gemm_ex(fmt, dev(c["x16"]), dev(c["scales"]), moved(c["w"]), 150, w2=moved(c["w2"]))
+    assert torch.equal(y, want)               # the same products in the same order, however the rows are fetched
+    assert ops.device_status() == 0
