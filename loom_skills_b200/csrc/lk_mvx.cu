@@ -820,7 +820,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (p.e.y_form != LK_Q8_ROWS) {
           if (in) store_elem(p.e.y, p.e.y_form, int64_t(t0 + tk) * p.n + n, v);
         } else if (kOut % 32 == 0) {
-          if (tk < ntok)   // n % 32 == 0: a warp is a whole group of one token
+          if (in)   // n % 32 == 0: a warp is a whole group of one token, inside or past the last output
             store_q8(static_cast<uint8_t*>(p.e.y), int64_t(p.tokens) * p.n, int64_t(t0 + tk) * p.n + n, v, lane);
         } else if (i == 0) {
           first[tk * 16 + r] = v;   // the unit's second tile finishes the group

@@ -257,3 +257,18 @@ def test_refusals(ops):
             ops.mv_q8_ex("q4_k", w, xq, **kw)
     with pytest.raises(ops.L.LkError):
         ops.mv_q8_ex("q3_k", torch.zeros(64 * 220, dtype=torch.uint8, device="cuda"), xq, 64, 512, 2)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("n", [4768, 9504])
+@pytest.mark.parametrize("tokens", [1, 3, 8, 17, 32])
+def test_q8_output_of_a_half_filled_last_tile(ops, fmt, n, tokens):
+    """Outputs that end in the middle of a 64-row tile: the groups past the last one are nobody's, not the next token's."""
+    k = 512
+    c = case(fmt, n, k, tokens, 31)
+    size = tokens * n + tokens * (n // 32) * 8
+    buf = torch.full((size + 256,), 9, dtype=torch.uint8, device="cuda")
+    run(ops, c, out="q8", y=buf)
+    assert (buf[size:] == 9).all()
+    assert torch.equal(buf[:size], ops.quant_q8(run(ops, c)))
+    assert ops.device_status() == 0
