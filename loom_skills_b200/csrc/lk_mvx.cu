@@ -29,6 +29,7 @@
 #include "lk_epi.cuh"
 #include "lk_formats.cuh"
 #include "lk_internal.h"
+#include "lk_rings.cuh"
 
 namespace lk {
 
@@ -37,59 +38,17 @@ int make_map(CUtensorMap* map, const void* base, CUtensorMapDataType dt, int ele
 
 namespace {
 
-constexpr int kRows = 32;              // weight rows of a warp
-constexpr int kSlices = 8;             // k slices of a stage, a warp of each group for each
-constexpr int kCWarps = 2 * kSlices;   // consumer warps
+using namespace mvx;
+
 // 16 consumer warps and a warpgroup whose first warp is the producer: launched at 96 registers a thread (the most that 640
 // threads can have), of which the producer's 128 threads give 64 each to the consumers' 512 (61440 in all, before and
 // after). The consumers' loop needs about 110: with 96 and a lone producer warp, spills cost 5% (Q4_K) to 30% (Q6_K).
 constexpr int kThreads = 32 * kCWarps + 128, kLaunchRegs = 96, kProducerRegs = 32, kConsumerRegs = 112;
 static_assert(128 * kProducerRegs + 32 * kCWarps * kConsumerRegs <= kThreads * kLaunchRegs, "a split that waits forever");
-constexpr int kTokStride = 36;         // floats between tokens of the partial sums: conflict-free stores
-constexpr int kSmemMax = 227 * 1024;
-constexpr int kMaxStages = 8;
 constexpr uint32_t kWaitPolls = 1u << 22;
 
 LK_DEV void mx_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 LK_DEV void mx_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
-// How a call's operands reach shared memory, and its tokens: kBox1 is the box form of one token, whose codes need no
-// swizzle (all rows read the same words) and come by plain bulk copies.
-enum { kRowForm = 0, kBox = 1, kBox1 = 2 };
-// packed bytes of a row's stage; 128-byte segments that can hold them wherever they start
-__host__ __device__ constexpr int stage_bytes(int fmt, int v) { return v / fmt_qk(fmt) * fmt_block_bytes(fmt); }
-__host__ __device__ constexpr int segments(int fmt, int v) {
-  return stage_bytes(fmt, v) % 128 == 0 ? stage_bytes(fmt, v) / 128 : (stage_bytes(fmt, v) + 126) / 128 + 1;
-}
-// row form slots: 16 bytes past a multiple of 128, so that 8 rows x 4 words fall into 32 banks; with room for a window's
-// 15 leading bytes and a realigning load's trailing word
-__host__ __device__ constexpr int slot_of(int bytes) { return (bytes + 32 + 111) / 128 * 128 + 16; }
-// weight bytes of a stage in shared memory, and a stage's activations (box forms: multiples of 1024, which the swizzle's
-// pattern is aligned to)
-__host__ __device__ constexpr int w_bytes(int fmt, int form, int rg, int v) {
-  return rg * kRows * (form == kRowForm ? slot_of(stage_bytes(fmt, v)) : segments(fmt, v) * 128);
-}
-__host__ __device__ constexpr int x_bytes(int form, int nt, int v) {
-  return form == kRowForm ? 8 * nt * (slot_of(v) + slot_of(v / 4)) : form == kBox1 ? (v + v / 4 + 1023) / 1024 * 1024 : 8 * nt * (v + v / 4);
-}
-// partial sums of all 16 warps; for 32 tokens of half of them, to which the other half adds
-constexpr int red_slices(int nt) { return nt <= 2 ? kCWarps : kCWarps / 2; }
-constexpr int red_bytes(int nt) { return red_slices(nt) * 8 * nt * kTokStride * 4; }
-constexpr int kTailBytes = 256 + 16 * 32 * 4;   // barriers; the first tile of a unit of two (q8 output of a pair)
-constexpr int fixed_bytes(int nt) { return 1024 + red_bytes(nt) + kTailBytes; }
-constexpr bool two_stages(int fmt, int form, int rg, int nt, int v) {
-  return 2 * (w_bytes(fmt, form, rg, v) + x_bytes(form, nt, v)) + fixed_bytes(nt) <= kSmemMax;
-}
-// values of a stage: 2048 for up to 8 tokens where two such stages fit (a stage's waits and addresses cost a warp as much as
-// a third of its 128 values' work: 16.9 -> 16.1 us on the Q4_K pair of 4096 -> 12288 at 8 tokens), else 1024. The same in
-// both forms of one row group, so that those sum in the same order.
-constexpr int stage_values(int fmt, int form, int rg, int nt) {
-  return nt == 1 && (rg == 1 || two_stages(fmt, form, rg, nt, 2048)) ? 2048 : 1024;
-}
-// whether two stages of 64-row tiles fit beside the sums
-constexpr bool two_groups(int fmt, int form, int nt) {
-  return form != kRowForm && two_stages(fmt, form, 2, nt, stage_values(fmt, form, 2, nt));
-}
 
 struct MvxArgs {
   int n, k, tokens;
@@ -561,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < kS; ++i) {
       mbar_init(&full[i], 2);   // the weights' bytes and the activations' are announced apart
-      mbar_init(&empty[i], RG * kSlices);   // the warps that read the stage
+      mbar_init(&empty[i], releases(RG, kS));
     }
     fence_mbar_init();
   }
@@ -717,7 +676,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       };
       for (int st = 0; st < nst && live; ++st) {
-        if (RG == 1 && ((st + round) & 1) != group) {   // the other group's; swapping the groups swaps two summands
+        const bool mine = takes(RG, group, st, round);
+        if (!mine && !follows(RG, kS)) {
           next();
           continue;
         }
@@ -725,6 +685,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           atomicOr(&g_status, 1u);
           live = false;
           break;
+        }
+        if (!mine) {
+          if (lane == 0) mbar_arrive(&empty[s]);
+          next();
+          continue;
         }
         const uint32_t sb = sbase + s * slot, xb = p.resident ? xbase + st * kXB : sb + kWB;
         const int gst = min(kV / 32, groups - st * (kV / 32));
@@ -848,16 +813,13 @@ struct Maps {
 
 template <int FMT, int FORM, bool PAIR, int NT, int RG>
 int launch(const Maps& m, MvxArgs a, cudaStream_t s) {
-  constexpr int kV = stage_values(FMT, FORM, RG, NT), kWB = w_bytes(FMT, FORM, RG, kV), kXB = x_bytes(FORM, NT, kV);
-  constexpr int kFixed = fixed_bytes(NT);
-  static_assert(2 * (kWB + kXB) + kFixed <= kSmemMax, "two stages at least");
+  constexpr int kV = stage_values(FMT, FORM, RG, NT), kXB = x_bytes(FORM, NT, kV);
+  static_assert(two_stages(FMT, FORM, RG, NT, kV), "two stages at least");
   static_assert(2 * kMaxStages * 8 <= 256, "the barriers");
-  const int nst = (a.k + kV - 1) / kV;
-  // the activations stay where they leave three stages of weights (two for the widest rows of 8 tokens and fewer)
-  a.resident = FORM != kRowForm && int64_t(nst) * kXB + (NT == 1 ? 2 : 3) * kWB + kFixed <= kSmemMax;
-  const int room = kSmemMax - kFixed - (a.resident ? nst * kXB : 0), slot = kWB + (a.resident ? 0 : kXB);
-  a.stages = room / slot < kMaxStages ? room / slot : kMaxStages;
-  const int smem = kFixed + a.stages * slot + (a.resident ? nst * kXB : 0);
+  const Ring ring = ring_of(FMT, FORM, RG, NT, a.k);
+  a.resident = ring.resident;
+  a.stages = ring.stages;
+  const int smem = fixed_bytes(NT) + ring.stages * ring.slot + (ring.resident ? ring.nst * kXB : 0);
   auto kern = k_mvx<FMT, FORM, PAIR, NT, RG>;
   static std::atomic<unsigned> allowed{0};
   if (!allow_smem(kern, kSmemMax, allowed)) return LK_ECUDA;

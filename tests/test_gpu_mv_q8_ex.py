@@ -272,3 +272,30 @@ def test_q8_output_of_a_half_filled_last_tile(ops, fmt, n, tokens):
     assert (buf[size:] == 9).all()
     assert torch.equal(buf[:size], ops.quant_q8(run(ops, c)))
     assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("fmt,n,k,tokens", [("q8_0", 4096, 4096, 12), ("q4_k", 4096, 14336, 8), ("q4_0", 2048, 8192, 3),
+                                            ("iq4_nl", 1500, 13824, 5), ("q4_k", 4096, 5120, 16), ("q6_k", 4096, 8192, 10),
+                                            ("q5_0", 2048, 11008, 6), ("q5_k", 1024, 14336, 2), ("iq4_xs", 1024, 8192, 7),
+                                            ("q5_0", 600, 4640, 4), ("q6_k", 600, 5376, 1)])
+def test_rings_whose_slots_change_groups(ops, fmt, n, k, tokens):
+    """More stages than an odd number of slots, while another stream keeps the memory busy: bit for bit the quiet result."""
+    c = case(fmt, n, k, tokens, 33)
+    w, xq = dev(c["w"]), xq_of(c)
+    call = lambda: ops.mv_q8_ex(fmt, w, xq, n, k, tokens)  # noqa: E731
+    want = call()
+    rows = np.arange(0, n, 41)
+    d = dict(c, w=c["w"][rows])
+    v, ev = ref(d)
+    ok, far = E.within(want[:, torch.from_numpy(rows).cuda()].double().cpu().numpy(), v, ev, "f32")
+    assert ok, far
+    a, b = (torch.empty(256 << 20, dtype=torch.uint8, device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    busy = torch.cuda.Stream()
+    with torch.cuda.stream(busy):
+        for _ in range(100):
+            b.copy_(a)
+    got = [call() for _ in range(200)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want) for y in got)
+    assert ops.device_status() == 0
