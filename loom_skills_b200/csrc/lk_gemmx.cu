@@ -28,6 +28,7 @@
 #include "lk_common.cuh"
 #include "lk_epi.cuh"
 #include "lk_internal.h"
+#include "lk_rings.cuh"
 #include "lk_stage.cuh"
 
 namespace lk {
@@ -39,11 +40,8 @@ int encode_tiled(CUtensorMap* map, CUtensorMapDataType dt, int rank, const void*
 
 namespace {
 
-constexpr int kRows = 128;       // weight rows of a CTA's tile (the M side)
-constexpr int kStageK = 64;      // k values per MMA stage: one 128-byte swizzled row
-constexpr int kEpW = 4;
-constexpr int kABytes = kRows * kStageK * 2;
-constexpr int kSmemMax = 227 * 1024;
+using namespace gx;
+
 constexpr uint32_t kWaitPolls = 1u << 22;
 
 struct GxArgs {
@@ -66,37 +64,6 @@ struct GxArgs {
 struct WeightMaps {
   CUtensorMap w[8], w2[8];
 };
-
-// Staging warps: groups of 8 that take the stages in turn.
-constexpr int kDqG = 2;
-constexpr int kThreads = 32 * (4 + 8 * kDqG + kEpW);
-
-// Two rings: stages (a staged weight tile and a token tile, one barrier for both, so the MMA warp waits once a stage) and
-// packed chunks. Few tokens: the weights stream from HBM once, and the packed ring gets what keeps that many bytes in
-// flight (110 KB a SM for the 4-bit formats); many: both operands come from L2 and the stages get it.
-constexpr int kTailBytes = 2 * 256 * 4 + 512;   // token scales of two tiles, barriers, the TMEM address
-struct Rings {
-  int s, r, b_bytes, raw_bytes;
-  constexpr int bytes() const { return s * (kABytes + b_bytes) + r * raw_bytes; }
-};
-constexpr int at_most(int a, int b) { return a < b ? a : b; }
-constexpr Rings rings_of(int fmt, bool win, int cg, int nt) {
-  Rings g{0, 0, nt / cg * kStageK * 2, kRows * row_slot_bytes(fmt, win)};
-  const int room = kSmemMax - 1024 - kTailBytes;
-  if (cg == 2) {
-    g.r = at_most(3, (room - 3 * (kABytes + g.b_bytes)) / g.raw_bytes);
-    g.s = at_most(6, (room - g.r * g.raw_bytes) / (kABytes + g.b_bytes));
-  } else {
-    g.r = at_most(nt <= 64 ? 5 : 3, (room - 3 * (kABytes + g.b_bytes)) / g.raw_bytes);
-    g.s = at_most(6, (room - g.r * g.raw_bytes) / (kABytes + g.b_bytes));
-  }
-  return g;
-}
-// the partial sums of a split reuse the rings: splits x ceil(nt / 8 / splits) groups of 8 tokens, at most 7 more than nt / 8
-constexpr int body_bytes(int fmt, bool win, int cg, int nt) {
-  const int ring = rings_of(fmt, win, cg, nt).bytes(), part = cg == 1 ? (nt + 56) * kRows * 4 : 0;
-  return ring > part ? ring : part;
-}
 
 LK_DEV void gx_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 LK_DEV void gx_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
@@ -396,7 +363,7 @@ template <int FMT, bool WIN, bool PAIR, int CG, int NT>
 __global__ void __launch_bounds__(kThreads, 1)
     k_gemmx(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ WeightMaps wm, const GxArgs p) {
   constexpr Rings kG = rings_of(FMT, WIN, CG, NT);
-  constexpr int kB = kG.b_bytes, kRaw = kG.raw_bytes, kS = kG.s, kR = kG.r, kBatch = kS >= 5 ? 2 : 1;
+  constexpr int kB = kG.b_bytes, kRaw = kG.raw_bytes, kS = kG.s, kR = kG.r, kBatch = batch_of(kS);
   constexpr int kRW = row_slot_bytes(FMT, WIN);
   constexpr int kCB = WIN ? chunk_bytes(FMT) : kChunkBytes;
   constexpr int kBuf = 2;                                // accumulators
@@ -636,13 +603,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           chunk += src & 15;
         }
         wait_for(&full_r[ar.s], ar.turn, live);
-        // this group's two stages of the chunk: subs 2 group, 2 group + 1, both sets of packed words loaded before either
-        // is decoded (a wait that is already satisfied still takes 100 to 250 clocks here, and one item's dependent
-        // chain about 500); or, where the ring is too short for that, every other stage by itself
+        // this group's stages of the chunk. Both sets of packed words are loaded before either is decoded (a wait that is
+        // already satisfied still takes 100 to 250 clocks here, and one item's dependent chain about 500); or, where the
+        // ring is too short for that, every other stage by itself
+        const Turn turn = turn_of(kBatch, group, WIN ? subs : 4);
         if (kBatch == 2) {
-          const int sub = 2 * group;
-          if (sub < subs) {
-            const bool two = sub + 1 < subs;
+          if (turn.count > 0) {
+            const int sub = turn.first;
+            const bool two = turn.count == 2;
             const Place<kS> st = at.ahead(sub), su = at.ahead(sub + 1);
             uint8_t* d0 = sA + st.s * kABytes;
             uint8_t* d1 = sA + su.s * kABytes;
@@ -673,8 +641,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         } else {
 #pragma unroll
-          for (int sub = 0; sub < 4; ++sub) {
-            if (sub % kDqG != group || sub >= subs) continue;
+          for (int i = 0; i < 2; ++i) {
+            if (i >= turn.count) break;
+            const int sub = turn.first + 2 * i;
             const Place<kS> st = at.ahead(sub);
             if (used + sub >= kS) wait_for(&empty[st.s], st.turn ^ 1, live);
             if (!live) break;

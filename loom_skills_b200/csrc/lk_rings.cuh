@@ -6,6 +6,7 @@
 // for the next one.
 #pragma once
 #include "lk_formats.cuh"
+#include "lk_stage.cuh"
 
 namespace lk {
 
@@ -88,5 +89,65 @@ __host__ __device__ constexpr bool follows(int rg, int stages) { return rg == 1 
 __host__ __device__ constexpr int releases(int rg, int stages) { return rg == 2 || follows(rg, stages) ? kCWarps : kSlices; }
 
 }  // namespace mvx
+
+// ---------------------------------------------------------------------------------------------------------------
+// lk_gemmx.cu: a ring of stages of 64 k (a staged weight tile and a token tile) and one of packed chunks of 256
+// ---------------------------------------------------------------------------------------------------------------
+namespace gx {
+
+constexpr int kRows = 128;       // weight rows of a CTA's tile (the M side)
+constexpr int kStageK = 64;      // k values per MMA stage: one 128-byte swizzled row
+constexpr int kEpW = 4;          // epilogue warps
+constexpr int kABytes = kRows * kStageK * 2;
+constexpr int kSmemMax = 227 * 1024;
+
+// Staging warps: groups of 8 that take the stages in turn.
+constexpr int kDqG = 2;
+constexpr int kThreads = 32 * (4 + 8 * kDqG + kEpW);
+
+// Two rings: stages (a staged weight tile and a token tile, one barrier for both, so the MMA warp waits once a stage) and
+// packed chunks. Few tokens: the weights stream from HBM once, and the packed ring gets what keeps that many bytes in
+// flight (110 KB a SM for the 4-bit formats); many: both operands come from L2 and the stages get it.
+constexpr int kTailBytes = 2 * 256 * 4 + 512;   // token scales of two tiles, barriers, the TMEM address
+struct Rings {
+  int s, r, b_bytes, raw_bytes;
+  __host__ __device__ constexpr int bytes() const { return s * (kABytes + b_bytes) + r * raw_bytes; }
+};
+__host__ __device__ constexpr int at_most(int a, int b) { return a < b ? a : b; }
+__host__ __device__ constexpr Rings rings_of(int fmt, bool win, int cg, int nt) {
+  Rings g{0, 0, nt / cg * kStageK * 2, kRows * row_slot_bytes(fmt, win)};
+  const int room = kSmemMax - 1024 - kTailBytes;
+  if (cg == 2) {
+    g.r = at_most(3, (room - 3 * (kABytes + g.b_bytes)) / g.raw_bytes);
+    g.s = at_most(6, (room - g.r * g.raw_bytes) / (kABytes + g.b_bytes));
+  } else {
+    g.r = at_most(nt <= 64 ? 5 : 3, (room - 3 * (kABytes + g.b_bytes)) / g.raw_bytes);
+    g.s = at_most(6, (room - g.r * g.raw_bytes) / (kABytes + g.b_bytes));
+  }
+  return g;
+}
+// the partial sums of a split reuse the rings: splits x ceil(nt / 8 / splits) groups of 8 tokens, at most 7 more than nt / 8
+__host__ __device__ constexpr int body_bytes(int fmt, bool win, int cg, int nt) {
+  const int ring = rings_of(fmt, win, cg, nt).bytes(), part = cg == 1 ? (nt + 56) * kRows * 4 : 0;
+  return ring > part ? ring : part;
+}
+
+// The stages of a chunk of `subs` (4, fewer in a row's last chunk) that a staging group takes: `count` from `first`, next to
+// each other with a batch of 2 (every other one with a batch of 1). A group waits for the slot of its last stage (batch 2;
+// of each stage, batch 1), which says that the MMAs up to the slot's last use are done; for its next wait to find the
+// barrier no more than one phase behind, its waits must be at most the ring's length apart. With a batch of 2 they
+// are up to 5 stages apart (group 1 around a last chunk of 1), because a last chunk of 2 is shared: taken whole by group 0
+// it would leave group 1 6 stages without a wait. With a batch of 1, up to 3.
+__host__ __device__ constexpr int batch_of(int stages) { return stages >= 5 ? 2 : 1; }
+struct Turn {
+  int first, count;
+};
+__host__ __device__ constexpr Turn turn_of(int batch, int group, int subs) {
+  if (batch == 2 && subs > 2) return Turn{2 * group, at_most(2, subs - 2 * group)};
+  if (batch == 2) return Turn{group, group < subs ? 1 : 0};
+  return Turn{group, (subs - group + 1) / 2};
+}
+
+}  // namespace gx
 
 }  // namespace lk

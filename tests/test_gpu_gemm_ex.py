@@ -226,3 +226,32 @@ def test_weights_off_the_16_byte_boundary(ops, fmt, k, off):
     y = ops.gemm_ex(fmt, dev(c["x16"]), dev(c["scales"]), moved(c["w"]), 150, w2=moved(c["w2"]))
     assert torch.equal(y, want)               # the same products in the same order, however the rows are fetched
     assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("fmt,rows,k,n,pair", [("q4_0", 2048, 896, 4864, False), ("iq4_nl", 1500, 2688, 9000, True),
+                                               ("mxfp4", 2048, 384, 6000, False), ("q4_0", 60, 896, 40000, False),
+                                               ("iq4_nl", 120, 384, 60000, True), ("q5_0", 30, 640, 60000, False),
+                                               ("mxfp4", 64, 2432, 30000, False), ("q8_0", 1024, 896, 4000, True)])
+def test_rows_that_end_in_a_chunk_of_two_stages(ops, fmt, rows, k, n, pair):
+    """Several tiles a cluster and k % 256 == 128, while another stream keeps the memory busy: bit for bit the quiet result."""
+    c = case(fmt, rows, k, n, 51, pair=pair)
+    x, sc, w = dev(c["x16"]), dev(c["scales"]), dev(c["w"])
+    w2 = dev(c["w2"]) if pair else None
+    call = lambda: ops.gemm_ex(fmt, x, sc, w, n, w2=w2)  # noqa: E731
+    want = call()
+    cols = np.arange(0, n, 61)
+    g, eg = E.product_f16(fmt, c["w"][cols], c["x16"], c["scales"], k)
+    u, eu = E.product_f16(fmt, c["w2"][cols], c["x16"], c["scales"], k) if pair else (None, None)
+    v, ev = E.epilogue(g, eg, "silu" if pair else "none", u, eu)
+    ok, far = E.within(want[:, torch.from_numpy(cols).cuda()].double().cpu().numpy(), v, ev, "f32")
+    assert ok, far
+    a, b = (torch.empty(256 << 20, dtype=torch.uint8, device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    busy = torch.cuda.Stream()
+    with torch.cuda.stream(busy):
+        for _ in range(100):
+            b.copy_(a)
+    for _ in range(60):
+        assert torch.equal(call(), want)
+    torch.cuda.synchronize()
+    assert ops.device_status() == 0

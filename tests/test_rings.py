@@ -28,3 +28,13 @@ def test_decode_rings(walk):
 def test_the_walk_finds_groups_that_do_not_follow_each_other(walk):
     r = walk("mvx", "alone")
     assert r.returncode == 1 and "another use" in r.stdout, r.stdout
+
+
+def test_prefill_rings(walk):
+    r = walk("gemmx")
+    assert r.returncode == 0, r.stdout
+
+
+def test_the_walk_finds_a_short_last_chunk_of_one_group(walk):
+    r = walk("gemmx", "whole")
+    assert r.returncode == 1 and "another use" in r.stdout, r.stdout
