@@ -669,30 +669,34 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp >= kEp0 && (CG == 2 || p.splits == 1)) {
     // ------------------------------------------------------------------ epilogue from TMEM
     const int q = warp & 3, row = 32 * q + lane;   // the lane quarter a warp may read
-    for (int li = 0; li < my_tiles && live; ++li) {
-      int t0, n0;
-      tile_of(cluster + li * nclusters, t0, n0);
-      const int buf = li % kBuf;
-      float* sc = stok + (li & 1) * 256;
-      for (int i = threadIdx.x - 32 * kEp0; i < NT; i += 32 * kEpW)
-        sc[i] = t0 + i < p.rows ? __ldg(p.scales + 2 * int64_t(t0 + i) + 1) : 0.0f;
-      asm volatile("bar.sync 3, 128;" ::: "memory");   // the four epilogue warps
-      wait_for(&acc_full[buf], (li / kBuf) & 1, live);
-      if (!live) break;
-      tc_fence_after();
+    int t0, n0;
+    epilogue_tiles(
+        my_tiles, live,
+        [&](int li) {
+          tile_of(cluster + li * nclusters, t0, n0);
+          float* sc = stok + (li & 1) * 256;
+          for (int i = threadIdx.x - 32 * kEp0; i < NT; i += 32 * kEpW)
+            sc[i] = t0 + i < p.rows ? __ldg(p.scales + 2 * int64_t(t0 + i) + 1) : 0.0f;
+        },
+        [] { asm volatile("bar.sync 3, 128;" ::: "memory"); },   // the four epilogue warps
+        [&](int li) { wait_for(&acc_full[li % kBuf], (li / kBuf) & 1, live); },
+        [&](int li) {
+          const int buf = li % kBuf;
+          const float* sc = stok + (li & 1) * 256;
+          tc_fence_after();
 #pragma unroll 1
-      for (int c = 0; c < NT && t0 + c < p.rows; c += kC) {
-        float v[kC];
-        tmem_ld(tmem + buf * NT + c + (uint32_t(32 * q) << 16), v);
-        finish<PAIR, kC>(p, v, sc + c, t0 + c, n0, row);
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if (CG == 2) arrive_at(peer_addr(&acc_empty[buf], 0));
-        else mbar_arrive(&acc_empty[buf]);
-      }
-    }
+          for (int c = 0; c < NT && t0 + c < p.rows; c += kC) {
+            float v[kC];
+            tmem_ld(tmem + buf * NT + c + (uint32_t(32 * q) << 16), v);
+            finish<PAIR, kC>(p, v, sc + c, t0 + c, n0, row);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if (CG == 2) arrive_at(peer_addr(&acc_empty[buf], 0));
+            else mbar_arrive(&acc_empty[buf]);
+          }
+        });
   }
   __syncwarp();
 

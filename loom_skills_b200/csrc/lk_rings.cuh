@@ -148,6 +148,20 @@ __host__ __device__ constexpr Turn turn_of(int batch, int group, int subs) {
   return Turn{group, (subs - group + 1) / 2};
 }
 
+// An epilogue warp's tiles: the four warps share the token scales that fill() loads, so each comes to sync() once a tile,
+// also after its own wait() has given up (live is false then) while another warp's passed.
+#pragma nv_exec_check_disable
+template <class Fill, class Sync, class Wait, class Work>
+__host__ __device__ __forceinline__ void epilogue_tiles(int tiles, const bool& live, const Fill& fill, const Sync& sync,
+                                                        const Wait& wait, const Work& work) {
+  for (int li = 0; li < tiles; ++li) {
+    fill(li);
+    sync();
+    if (live) wait(li);
+    if (live) work(li);
+  }
+}
+
 }  // namespace gx
 
 }  // namespace lk

@@ -6,6 +6,7 @@
 // Planted mistakes, for the test of the walk:
 //   ring_walk mvx [alone]     alone: the groups never follow each other's stages
 //   ring_walk gemmx [whole]   whole: a last chunk of two stages is group 0's alone
+//   ring_walk epilogue        waits that give up in some of the epilogue warps
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -356,11 +357,31 @@ int run_gemmx(bool whole) {
   return faults != 0;
 }
 
+// Each warp meets the others once a tile, whichever of its waits gives up, and neither waits nor works after that.
+int run_epilogue() {
+  for (int tiles = 0; tiles <= 6; ++tiles)
+    for (int gives_up = 0; gives_up <= tiles; ++gives_up) {   // at this tile; at `tiles`: never
+      bool live = true;
+      int fills = 0, syncs = 0, waits = 0, works = 0;
+      lk::gx::epilogue_tiles(
+          tiles, live, [&](int li) { fills += li == syncs; }, [&] { ++syncs; },
+          [&](int li) {
+            ++waits;
+            if (li == gives_up) live = false;
+          },
+          [&](int li) { works += li == waits - 1; });
+      if (fills != tiles || syncs != tiles || works != gives_up || waits != (gives_up < tiles ? gives_up + 1 : tiles))
+        return printf("%d tiles, given up at %d: %d barriers, %d waits, %d tiles finished\n", tiles, gives_up, syncs, waits, works), 1;
+    }
+  return 0;
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
   const bool plant = argc > 2;
   if (argc > 1 && !strcmp(argv[1], "mvx")) return run_mvx(plant);
   if (argc > 1 && !strcmp(argv[1], "gemmx")) return run_gemmx(plant);
+  if (argc > 1 && !strcmp(argv[1], "epilogue")) return run_epilogue();
   return 2;
 }

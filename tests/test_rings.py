@@ -38,3 +38,8 @@ def test_prefill_rings(walk):
 def test_the_walk_finds_a_short_last_chunk_of_one_group(walk):
     r = walk("gemmx", "whole")
     assert r.returncode == 1 and "another use" in r.stdout, r.stdout
+
+
+def test_epilogue_warps_meet_after_a_wait_gave_up(walk):
+    r = walk("epilogue")
+    assert r.returncode == 0, r.stdout
