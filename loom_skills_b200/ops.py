@@ -828,6 +828,11 @@ def ffn(fmt, x, norm_w, w_gate, w_up, w_down, h, f, residual=None, eps=1e-6, act
     formats with integer codes): int8 activations, three launches -- norm to q8 codes, gate/up to q8 codes, down onto
     the stream. Prefill: norm to row-scaled f16, gate/up GEMM, row scale, down GEMM onto the stream; the activations
     between the two GEMMs are held in the stream's type. `prefill` forces either path."""
+    dev = _device(x, norm_w, w_gate, w_up, w_down, residual, b_gate, b_up, b_down)
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):   # for the row scale too, which takes the current device's stream
+            return ffn(fmt, x, norm_w, w_gate, w_up, w_down, h, f, residual, eps, act, b_gate, b_up, b_down, fmt_down,
+                       prefill, alpha, limit)
     tokens = x.shape[0]
     fd = fmt_down or fmt
     stream = x if residual is None else residual
