@@ -824,10 +824,11 @@ def ffn(fmt, x, norm_w, w_gate, w_up, w_down, h, f, residual=None, eps=1e-6, act
         s = x + residual;  v = rms_norm(s) * norm_w;  s + Wd (act(Wg v + b_gate) * (Wu v + b_up)) + b_down
     x [tokens][h] (the block before's output) and residual [tokens][h] (the stream; None: x is the stream), f32, f16 or
     bf16; returns the new stream [tokens][h] in the stream's type. w_gate, w_up: f rows of h values in fmt; w_down: h
-    rows of f values in fmt_down or fmt. Decode (fewer than 64 tokens, the reference's switch, gen_llm.py:6107, and
-    formats with integer codes): int8 activations, three launches -- norm to q8 codes, gate/up to q8 codes, down onto
-    the stream. Prefill: norm to row-scaled f16, gate/up GEMM, row scale, down GEMM onto the stream; the activations
-    between the two GEMMs are held in the stream's type. `prefill` forces either path."""
+    rows of f values in fmt_down or fmt. Decode (formats with integer codes, and fewer than 64 tokens -- the reference's
+    switch, gen_llm.py:6107 -- or an h or f that is no multiple of 64, which the GEMM does not take): int8 activations,
+    three launches -- norm to q8 codes, gate/up to q8 codes, down onto the stream. Prefill: norm to row-scaled f16, gate/up
+    GEMM, row scale, down GEMM onto the stream; the activations between the two GEMMs are held in the stream's type.
+    `prefill` forces either path."""
     dev = _device(x, norm_w, w_gate, w_up, w_down, residual, b_gate, b_up, b_down)
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):   # for the row scale too, which takes the current device's stream
@@ -837,7 +838,8 @@ def ffn(fmt, x, norm_w, w_gate, w_up, w_down, h, f, residual=None, eps=1e-6, act
     fd = fmt_down or fmt
     stream = x if residual is None else residual
     if prefill is None:
-        prefill = tokens >= 64 or _fmt(fmt) not in _Q8_FORMATS or _fmt(fd) not in _Q8_FORMATS
+        codes = _fmt(fmt) in _Q8_FORMATS and _fmt(fd) in _Q8_FORMATS
+        prefill = not codes or (tokens >= 64 and h % 64 == 0 and f % 64 == 0)
     ep = dict(w2=w_up, bias=b_gate, bias2=b_up, act=act, alpha=alpha, limit=limit)
     form = "row_f16" if prefill else "q8"
     v, s = rms_norm(x, norm_w, eps, residual=residual, form=form) if residual is not None else \

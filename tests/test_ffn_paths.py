@@ -53,3 +53,13 @@ def test_every_call_runs_on_the_tensors_device(block, on, prefill, residual):
     assert [c[0] for c in calls] == names
     assert all(c[1] == on for c in calls)
     assert torch.cuda.current_device() == 0
+
+
+@pytest.mark.parametrize("fmt,tokens,h,f,kw,prefill", [
+    ("q4_0", 63, 128, 64, {}, False), ("q4_0", 64, 128, 64, {}, True), ("q3_k", 1, 256, 256, {}, True),
+    # widths that the GEMM does not take
+    ("q4_0", 64, 96, 64, {}, False), ("q8_0", 200, 128, 160, {}, False), ("q4_0", 64, 96, 256, dict(fmt_down="q4_k"), False),
+    ("mxfp4", 4, 96, 64, {}, True), ("q4_0", 64, 96, 64, dict(prefill=True), True)])
+def test_which_path(block, fmt, tokens, h, f, kw, prefill):
+    calls = block(tokens, h, f, fmt=fmt, **kw)
+    assert ("gemm_ex" in [c[0] for c in calls]) == prefill

@@ -182,3 +182,17 @@ def test_formats_by_id(ops):
     by_name = ops.ffn("q4_k", x, nw, w, w, w, 256, 256)
     assert torch.equal(ops.ffn(ops.L.Q4_K, x, nw, w, w, w, 256, 256), by_name)
     assert torch.equal(ops.ffn("q4_k", x, nw, w, w, w, 256, 256, prefill=False), by_name)
+
+
+@pytest.mark.parametrize("fmt", ["q4_0", "iq4_nl"])
+@pytest.mark.parametrize("tokens", [64, 100])
+@pytest.mark.parametrize("h,f", [(96, 160), (96, 128), (128, 224)])
+def test_many_tokens_of_widths_that_are_no_multiple_of_64(ops, fmt, tokens, h, f):
+    rng = np.random.default_rng(tokens)
+    x, r = (dev(rng.standard_normal((tokens, h)).astype(np.float32)) for _ in range(2))
+    nw = np.ones(h, np.float32)
+    wg, wu, wd = weights(fmt, f, h, 1), weights(fmt, f, h, 2), weights(fmt, h, f, 3)
+    y = ops.ffn(fmt, x, dev(nw), dev(wg), dev(wu), dev(wd), h, f, residual=r)
+    ref = block_ref(fmt, x.double().cpu().numpy(), r.double().cpu().numpy(), nw, wg, wu, wd, h, f, "silu", 0, 0, 0, True)
+    assert O.rel_l2(y.double().cpu().numpy(), ref) <= 1e-3   # as test_block's f32 stream
+    assert ops.device_status() == 0
