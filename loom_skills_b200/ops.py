@@ -827,8 +827,8 @@ def ffn(fmt, x, norm_w, w_gate, w_up, w_down, h, f, residual=None, eps=1e-6, act
     rows of f values in fmt_down or fmt. Decode (formats with integer codes, and fewer than 64 tokens -- the reference's
     switch, gen_llm.py:6107 -- or an h or f that is no multiple of 64, which the GEMM does not take): int8 activations,
     three launches -- norm to q8 codes, gate/up to q8 codes, down onto the stream. Prefill: norm to row-scaled f16, gate/up
-    GEMM, row scale, down GEMM onto the stream; the activations between the two GEMMs are held in the stream's type.
-    `prefill` forces either path."""
+    GEMM, row scale, down GEMM onto the stream; the activations between the two GEMMs are held in bf16 for a bf16
+    stream, else in f32 (the row scale takes these two, and f16 would end at 65504). `prefill` forces either path."""
     dev = _device(x, norm_w, w_gate, w_up, w_down, residual, b_gate, b_up, b_down)
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):   # for the row scale too, which takes the current device's stream

@@ -63,3 +63,10 @@ def test_every_call_runs_on_the_tensors_device(block, on, prefill, residual):
 def test_which_path(block, fmt, tokens, h, f, kw, prefill):
     calls = block(tokens, h, f, fmt=fmt, **kw)
     assert ("gemm_ex" in [c[0] for c in calls]) == prefill
+
+
+@pytest.mark.parametrize("dtype,between", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32),
+                                           (torch.float32, torch.float32)])
+def test_the_type_between_the_gemms(block, dtype, between):
+    calls = [c for c in block(64, 128, 64, dtype=dtype) if c[0] == "gemm_ex"]
+    assert [c[2]["out_dtype"] for c in calls] == [between, dtype]
