@@ -1,5 +1,6 @@
 """Build liblk.so in-tree with nvcc for sm_100a (no torch extension machinery: the library is a plain C ABI)."""
 import os
+import re
 import subprocess
 import sys
 
@@ -12,6 +13,25 @@ SOURCES = ["lk_api.cu", "lk_dequant.cu", "lk_mv.cu", "lk_mvq8.cu","lk_gemm.cu", 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-Xcompiler", "-fPIC",
          "--expt-relaxed-constexpr", "-Xptxas", "-warn-spills"]
+
+
+# Registers a thread that a kernel must be launched with at least: k_mvx's consumer warps take theirs from the launch's
+# total, and a smaller one would leave them waiting (lk_mvx.cu, kLaunchRegs).
+LAUNCH_REGISTERS = {"lk_mvx.cu": ("k_mvx", 96)}
+
+
+def check_registers(src, ptxas):
+    """Holds the registers that ptxas -v reports for the kernels of `src` against LAUNCH_REGISTERS."""
+    if src not in LAUNCH_REGISTERS:
+        return
+    kernel, least = LAUNCH_REGISTERS[src]
+    names = re.findall(r"Compiling entry function '(\w+)'", ptxas)
+    used = [int(n) for n in re.findall(r"Used (\d+) registers", ptxas)]
+    if len(names) != len(used) or not any(kernel in n for n in names):
+        raise RuntimeError(f"{src}: ptxas reported no registers of {kernel}")
+    few = [n for n, r in zip(names, used) if kernel in n and r < least]
+    if few:
+        raise RuntimeError(f"{src}: fewer than {least} registers a thread in {', '.join(few)}")
 
 
 def _write_iq3s_grid(bdir):
@@ -53,7 +73,8 @@ def build(force=False, verbose=False, jobs=None):
     for src in SOURCES:
         obj = os.path.join(bdir, src.replace(".cu", ".o"))
         objs.append(obj)
-        cmd = [NVCC, *FLAGS, "-I", bdir, "-c", os.path.join(CSRC, src), "-o", obj]
+        check = ["-Xptxas", "-v"] if src in LAUNCH_REGISTERS else []
+        cmd = [NVCC, *FLAGS, *check, "-I", bdir, "-c", os.path.join(CSRC, src), "-o", obj]
         if verbose:
             print(" ".join(cmd), flush=True)
         procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
@@ -64,6 +85,8 @@ def build(force=False, verbose=False, jobs=None):
             sys.stdout.write(out)
         if p.returncode:
             failed.append(src)
+        else:
+            check_registers(src, out)
     if failed:
         raise RuntimeError("nvcc failed for " + ", ".join(failed))
     tmp = LIB + ".tmp"

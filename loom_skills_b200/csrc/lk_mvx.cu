@@ -43,6 +43,7 @@ using namespace mvx;
 // 16 consumer warps and a warpgroup whose first warp is the producer: launched at 96 registers a thread (the most that 640
 // threads can have), of which the producer's 128 threads give 64 each to the consumers' 512 (61440 in all, before and
 // after). The consumers' loop needs about 110: with 96 and a lone producer warp, spills cost 5% (Q4_K) to 30% (Q6_K).
+// The build holds every instantiation to the 96 (build.py): launched with fewer, the consumers' would never come free.
 constexpr int kThreads = 32 * kCWarps + 128, kLaunchRegs = 96, kProducerRegs = 32, kConsumerRegs = 112;
 static_assert(128 * kProducerRegs + 32 * kCWarps * kConsumerRegs <= kThreads * kLaunchRegs, "a split that waits forever");
 constexpr uint32_t kWaitPolls = 1u << 22;
@@ -823,11 +824,6 @@ int launch(const Maps& m, MvxArgs a, cudaStream_t s) {
   auto kern = k_mvx<FMT, FORM, PAIR, NT, RG>;
   static std::atomic<unsigned> allowed{0};
   if (!allow_smem(kern, kSmemMax, allowed)) return LK_ECUDA;
-  static const int regs = [&] {
-    cudaFuncAttributes fa;
-    return cudaFuncGetAttributes(&fa, kern) == cudaSuccess ? fa.numRegs : 0;
-  }();
-  if (regs < kLaunchRegs) return LK_ECUDA;   // the consumers' registers would never come free
   int dev = 0, sms = 0;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
