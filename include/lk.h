@@ -114,8 +114,8 @@ int lk_row_scale_f8(int rows, int k, const void* x, int x_dtype, float* scales, 
  *                     LK_E4M3      lk_row_scale_f8's x8 [rows][k], `scales` = its s8 [rows][2]; likewise
  * x [rows][k] of x_dtype, residual [rows][k] of r_dtype or NULL (then h must be NULL and r_dtype is not read), weight
  * [k] of w_dtype: each LK_F32, LK_F16 or LK_BF16. h may be the residual's buffer (the stream updated in place) or, of
- * x_dtype, x's; a plain y may be x's buffer when its type is x_dtype. No other two operands may overlap. Pointers are
- * aligned to their elements; 16-byte aligned operands with k % 8 == 0 are moved in 16-byte vectors. k <= 32768
+ * x_dtype, x's; a plain y may be x's buffer when its type is x_dtype. No output may overlap another operand in any other
+ * way (LK_EINVAL). Pointers are aligned to their elements; 16-byte aligned operands with k % 8 == 0 are moved in 16-byte vectors. k <= 32768
  * (LK_ERANGE beyond). The sum of squares is held in f32: a row whose |h| passes about 1e17 gives zeros. */
 int lk_rms_norm(int rows, int k, const void* x, int x_dtype, const void* residual, int r_dtype, const void* weight,
                 int w_dtype, float eps, void* h, int form, void* y, float* scales, lk_stream_t stream);
@@ -168,7 +168,8 @@ int lk_mv_q8_multi(int fmt, int nseg, const int* n, const void* const* w, float*
  * act: LK_ACT_NONE, _SILU, _GELU, _GELU_ERF or _RELU; with w2 also _SWIGLU_OAI (alpha, limit). bias, bias2: f32 [n] or
  * NULL (bias2 only with w2). residual: [tokens][n] of r_dtype (LK_F32, LK_F16, LK_BF16) or NULL. y_form: LK_F32, LK_F16
  * or LK_BF16, [tokens][n]; or LK_Q8_ROWS, lk_quant_q8's buffer of the tokens x n values (n % 32 == 0, y 16-byte aligned):
- * the next product's input. y may be the residual's buffer when both have the same type. xq, k and the formats as
+ * the next product's input. y may be the residual's buffer when both have the same type, and overlap no other operand
+ * (LK_EINVAL). xq, k and the formats as
  * lk_mv_q8 (every format with integer codes); w, w2 2-byte aligned. Any tokens from 0 to 2097120, any
  * n from 1 to 2^30 (LK_ERANGE beyond). */
 int lk_mv_q8_ex(int fmt, int n, int k, int tokens, const uint8_t* xq, const void* w, const void* w2, const float* bias,
@@ -206,7 +207,7 @@ int lk_gemm(int fmt, int mode, int rows, int k, int n, const uint16_t* x16, cons
  *   p[t][n] = scales[t][1] * sum_k x16[t][k] W16[n][k];  v = act(p + bias) or act(p + bias) * (p2 + bias2);  y = v + residual
  * W16: lk_gemm's f16 staging of every format it takes (one format for w and w2). The sums, bias, activation and residual
  * are f32; y is rounded once to y_dtype (LK_F32, LK_F16, LK_BF16). act, alpha, limit, biases and residual as lk_mv_q8_ex;
- * y may be the residual's buffer when both have the same type. x16, scales as lk_gemm (x16 16-byte aligned), k % 64 == 0
+ * y may be the residual's buffer when both have the same type, and overlap no other operand. x16, scales as lk_gemm (x16 16-byte aligned), k % 64 == 0
  * and a whole number of the format's blocks; any rows >= 0 and any n from 1 to 2^30 (LK_ERANGE beyond); w, w2 2-byte
  * aligned (ggml MXFP4: any). */
 int lk_gemm_ex(int fmt, int rows, int k, int n, const uint16_t* x16, const float* scales, const void* w, const void* w2,

@@ -37,6 +37,17 @@ static constexpr int kMaxOutputs = 1 << 30;   // outputs of an epilogue product:
 static bool plain_dtype(int dt) { return dt == LK_F32 || dt == LK_F16 || dt == LK_BF16; }
 static uintptr_t elem_bytes(int dt) { return dt == LK_F32 ? 4 : dt == LK_E4M3 ? 1 : 2; }
 
+// whether [a, a + na) and [b, b + nb) have bytes in common
+static bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a && b && x < y + uintptr_t(nb) && y < x + uintptr_t(na);
+}
+// bytes of `rows` rows of k values in a norm's or an epilogue's output form
+static int64_t form_bytes(int form, int64_t rows, int64_t k) {
+  return rows * k * (form == LK_Q8_ROWS || form == LK_E4M3 ? 1 : form == LK_F16_ROWS ? 2 : int64_t(elem_bytes(form))) +
+         (form == LK_Q8_ROWS ? rows * (k / 32) * 8 : 0);
+}
+
 // the epilogue operands shared by lk_mv_q8_ex and lk_gemm_ex
 static int epilogue_check(const void* w2, const float* bias, const float* bias2, int act, const void* residual,
                           int r_dtype, const void* y, int y_form) {
@@ -47,6 +58,16 @@ static int epilogue_check(const void* w2, const float* bias, const float* bias2,
   if (!aligned(bias, 4) || !aligned(bias2, 4) || (residual && !aligned(residual, elem_bytes(r_dtype)))) return LK_EALIGN;
   if (!aligned(y, y_form == LK_Q8_ROWS ? 16 : elem_bytes(y_form))) return LK_EALIGN;
   return LK_OK;
+}
+
+// whether an epilogue product's output lies over an operand that other outputs are still computed from (the residual's own
+// buffer: each output reads its own value and replaces it)
+static bool output_over_operand(const Epilogue& e, int64_t rows, int64_t n, const void* x, int64_t xb, const void* scales,
+                                const void* w, const void* w2, int64_t wb) {
+  const int64_t yb = form_bytes(e.y_form, rows, n);
+  return overlap(e.y, yb, x, xb) || overlap(e.y, yb, scales, rows * 8) || overlap(e.y, yb, w, wb) ||
+         overlap(e.y, yb, w2, wb) || overlap(e.y, yb, e.bias, n * 4) || overlap(e.y, yb, e.bias2, n * 4) ||
+         (e.res != e.y && e.res && overlap(e.y, yb, e.res, form_bytes(e.res_dtype, rows, n)));
 }
 
 extern "C" {
@@ -622,6 +643,15 @@ int lk_rms_norm(int rows, int k, const void* x, int x_dtype, const void* residua
   if (!aligned(x, elem_bytes(x_dtype)) || !aligned(weight, elem_bytes(w_dtype))) return LK_EALIGN;
   if (residual && (!aligned(residual, elem_bytes(r_dtype)) || !aligned(h, elem_bytes(r_dtype)))) return LK_EALIGN;
   if (!aligned(y, form == LK_Q8_ROWS ? 16 : elem_bytes(form)) || (scaled && !aligned(scales, 4))) return LK_EALIGN;
+  // outputs over anything but their own rows' inputs (h over the residual or x, y over x, from the same start)
+  const int64_t xb = form_bytes(x_dtype, rows, k), wb = form_bytes(w_dtype, 1, k), yb = form_bytes(form, rows, k);
+  const int64_t rb = residual ? form_bytes(r_dtype, rows, k) : 0, sb = scaled ? int64_t(rows) * 8 : 0;
+  const void* s = scaled ? scales : nullptr;
+  if ((y != x && overlap(y, yb, x, xb)) || overlap(y, yb, residual, rb) || overlap(y, yb, weight, wb) ||
+      overlap(y, yb, h, rb) || (h != x && overlap(h, rb, x, xb)) || (h != residual && overlap(h, rb, residual, rb)) ||
+      overlap(h, rb, weight, wb) || overlap(s, sb, x, xb) || overlap(s, sb, residual, rb) || overlap(s, sb, weight, wb) ||
+      overlap(s, sb, h, rb) || overlap(s, sb, y, yb))
+    return LK_EINVAL;
   return rms_norm(rows, k, x, x_dtype, residual, r_dtype, weight, w_dtype, eps, h, form, y, scales,
                   (cudaStream_t)stream);
 }
@@ -639,6 +669,8 @@ int lk_mv_q8_ex(int fmt, int n, int k, int tokens, const uint8_t* xq, const void
   if (!xq || !w || !y) return LK_EINVAL;
   if (!aligned(xq, 16) || !aligned(w, 2) || !aligned(w2, 2)) return LK_EALIGN;
   const Epilogue e{bias, bias2, residual, r_dtype, act, alpha, limit, y, y_form};
+  if (output_over_operand(e, tokens, n, xq, form_bytes(LK_Q8_ROWS, tokens, k), nullptr, w, w2, n * lk_row_bytes(fmt, k)))
+    return LK_EINVAL;
   return mv_q8_ex(fmt, n, k, tokens, xq, w, w2, e, (cudaStream_t)stream);
 }
 
@@ -655,6 +687,8 @@ int lk_gemm_ex(int fmt, int rows, int k, int n, const uint16_t* x16, const float
   if (!aligned(x16, 16) || !aligned(scales, 4)) return LK_EALIGN;
   if (fmt != LK_MXFP4 && (!aligned(w, 2) || !aligned(w2, 2))) return LK_EALIGN;
   const Epilogue e{bias, bias2, residual, r_dtype, act, alpha, limit, y, y_dtype};
+  if (output_over_operand(e, rows, n, x16, form_bytes(LK_F16, rows, k), scales, w, w2, n * lk_row_bytes(fmt, k)))
+    return LK_EINVAL;
   return gemm_ex(fmt, rows, k, n, x16, scales, w, w2, e, (cudaStream_t)stream);
 }
 

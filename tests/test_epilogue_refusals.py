@@ -89,3 +89,27 @@ def test_ops_take_cuda_tensors_only():
         ops.mv_q8_ex("q8_0", torch.zeros(4, 68, dtype=torch.uint8), q, 4, 64, 2)
     with pytest.raises(L.LkError):
         ops.gemm_ex("q8_0", x.half(), torch.ones(2, 2), torch.zeros(4, 68, dtype=torch.uint8), 4)
+
+
+# operands far apart, of the sizes that the calls below read and write
+FX, FW, FW2, FY, FR, FB, FS, FH = (i << 24 for i in range(1, 9))
+
+
+@pytest.mark.parametrize("at", [FX, FX + 64, FX + 2 * 256 - 256, FW, FW + 64 * 144 - 16, FW2, FB, FB + 128, FR + 256, FR - 256])
+def test_products_written_over_their_operands(at):
+    assert mv(xq=FX, w=FW, w2=FW2, b=FB, r=FR, y=at) == EINVAL
+    assert gemm(x=FX, w=FW, w2=FW2, b=FB, r=FR, s=FS, y=at) == EINVAL
+
+
+def test_a_product_written_over_its_input_rows():
+    assert mv(xq=FX, n=256, w=FW, y=FX, form=L.Q8_ROWS) == EINVAL
+    assert gemm(x=FX, s=FS, w=FW, y=FS) == EINVAL and gemm(x=FX, s=FS, w=FW, y=FX, form=L.F16) == EINVAL
+
+
+@pytest.mark.parametrize("kw", [
+    dict(y=FX + 16), dict(y=FX - 16), dict(y=FR), dict(y=FR + 128), dict(y=FW), dict(y=FH), dict(y=FH + 64), dict(h=FX + 64),
+    dict(h=FR + 64), dict(h=FW), dict(form=L.F16_ROWS, s=FX), dict(form=L.F16_ROWS, s=FR + 4), dict(form=L.E4M3, s=FW),
+    dict(form=L.E4M3, s=FH + 4), dict(form=L.E4M3, s=FY + 4)])
+def test_norms_written_over_their_operands(kw):
+    args = dict(x=FX, xd=L.BF16, r=FR, rd=L.BF16, w=FW, h=FH, y=FY, s=FS, form=L.BF16)
+    assert norm(**{**args, **kw}) == EINVAL
