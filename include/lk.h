@@ -15,6 +15,12 @@
  *    reference has no runtime errors (its contracts are index.assume preconditions); violating one here is an error
  *    code, not undefined behaviour. A CUDA launch error is LK_ECUDA.
  *  - Weight formats use the ggml type ids (gguf.GGMLQuantizationType).
+ *  - The decode products (lk_mv_q8*) and lk_moe_ffn_decode_q8 request their first packed weights before the kernel in front of
+ *    them on the stream has ended. A kernel that writes packed weights and lets its own dependents start early
+ *    (programmatic dependent launch) must therefore not be the one in front of them; copies, and kernels launched
+ *    without that attribute, may be.
+ *  - Copies move whole aligned 16-byte units: up to 15 bytes before or after an operand are read where its ends are not
+ *    at 16-byte boundaries (never another unit than one that holds the operand's own bytes), and never used.
  */
 #ifndef LK_H
 #define LK_H
@@ -115,8 +121,9 @@ int lk_row_scale_f8(int rows, int k, const void* x, int x_dtype, float* scales, 
  * x [rows][k] of x_dtype, residual [rows][k] of r_dtype or NULL (then h must be NULL and r_dtype is not read), weight
  * [k] of w_dtype: each LK_F32, LK_F16 or LK_BF16. h may be the residual's buffer (the stream updated in place) or, of
  * x_dtype, x's; a plain y may be x's buffer when its type is x_dtype. No output may overlap another operand in any other
- * way (LK_EINVAL). Pointers are aligned to their elements; 16-byte aligned operands with k % 8 == 0 are moved in 16-byte vectors. k <= 32768
- * (LK_ERANGE beyond). The sum of squares is held in f32: a row whose |h| passes about 1e17 gives zeros. */
+ * way (LK_EINVAL). Pointers are aligned to their elements; 16-byte aligned operands with k % 8 == 0 are moved in 16-byte
+ * vectors. k <= 32768 (LK_ERANGE beyond). The sum of squares is held in f32: a row whose |h| passes about 1e17 gives zeros, and with
+ * eps = 0 a row below about 1e-19 loses its squares (infinities below 1e-23, NaN where all of it is zero). */
 int lk_rms_norm(int rows, int k, const void* x, int x_dtype, const void* residual, int r_dtype, const void* weight,
                 int w_dtype, float eps, void* h, int form, void* y, float* scales, lk_stream_t stream);
 

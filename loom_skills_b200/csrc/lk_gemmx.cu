@@ -17,10 +17,13 @@
 //           tiles meet through distributed shared memory, each CTA finishing every S-th group of tokens. The order of
 //           the sum is fixed, so results repeat bit for bit, and nothing waits on a CTA that may not be running.
 //
-// Measured (device time, Q4_K): a gate / up pair of 2048 x 4096 x 2 12288 294 to 330 us (1.25 to 1.4 PFLOP/s by the clock the
-// power limit leaves; sustained cuBLAS bf16 is 1.42), 4096 x 12288 x 5120 440 to 470 us; IQ4_NL 4096 x 27648 x 5120 1065 us.
+// Measured (Q4_K, device time): a gate / up pair of 2048 x 4096 x 2 12288 309 to 320 us in a short burst from cold clocks (1.29 to
+// 1.33 PFLOP/s), 362 where calls follow one another for seconds and the power limit holds (1.14; sustained cuBLAS bf16 is 1.42);
+// IQ4_NL 4096 x 27648 x 5120 1028 to 1091 cold, 1170 sustained; the pair of 2048 rows in other formats (cold) IQ4_NL 338,
+// Q5_0 383, Q8_0 380 to 430, Q6_K 415 to 463, IQ4_XS 606, MXFP4 618, Q5_K 761, IQ3_S 1168, Q3_K 3540: staging, by the value where
+// the format has no word-wise decode.
 // Many tokens: a stage moves 74 KB through shared memory (about 580 clocks) for 512 clocks of MMA. Few: staging a stage of
-// weights and issuing its MMAs each take a warp 600 to 700 clocks of latency (64 x 4096 x 2 12288 53 us); more staging
+// weights and issuing its MMAs each take a warp 600 to 700 clocks of latency (64 x 4096 x 2 12288 47 to 55 us); more staging
 // warps, deeper rings and looking ahead of the MMA warp's waits gained nothing.
 //
 // Warps: 0 loads token tiles and 2 packed weights (TMA), 1 issues the MMAs, 4.. stage weights (packed chunk -> f16 in
@@ -177,16 +180,7 @@ LK_DEV void tfree(uint32_t addr, uint32_t cols) {
   else
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
 }
-// 32 lanes x 8 or 16 consecutive columns
-LK_DEV void tmem_ld(uint32_t addr, float (&v)[8]) {
-  uint32_t r[8];
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "r"(addr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
-}
+// 32 lanes x 16 consecutive columns
 LK_DEV void tmem_ld(uint32_t addr, float (&v)[16]) {
   uint32_t r[16];
   asm volatile(

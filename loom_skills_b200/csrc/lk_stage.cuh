@@ -137,9 +137,6 @@ LK_DEV void dequant_group_any(const uint8_t* chunk, int j, uint8_t* b_tile, int 
     *reinterpret_cast<uint4*>(b_tile + sw128(r, c0 + cc)) = reinterpret_cast<const uint4*>(h)[cc];
 }
 
-// 16-byte chunk `c` of row `r` of a K-major 128-byte-swizzled tile
-
-
 // 8 codes (bytes of t0, t1; low nibble only) -> 8 f16 (1024 + code), natural k order
 LK_DEV void magic8(uint32_t t0, uint32_t t1, uint32_t (&h)[4]) {
   h[0] = prmt(t0, 0x64646464u, 0x4140u);
