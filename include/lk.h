@@ -176,9 +176,8 @@ int lk_mv_q8_multi(int fmt, int nseg, const int* n, const void* const* w, float*
  * NULL (bias2 only with w2). residual: [tokens][n] of r_dtype (LK_F32, LK_F16, LK_BF16) or NULL. y_form: LK_F32, LK_F16
  * or LK_BF16, [tokens][n]; or LK_Q8_ROWS, lk_quant_q8's buffer of the tokens x n values (n % 32 == 0, y 16-byte aligned):
  * the next product's input. y may be the residual's buffer when both have the same type, and overlap no other operand
- * (LK_EINVAL). xq, k and the formats as
- * lk_mv_q8 (every format with integer codes); w, w2 2-byte aligned. Any tokens from 0 to 2097120, any
- * n from 1 to 2^30 (LK_ERANGE beyond). */
+ * (LK_EINVAL). xq, k and the formats as lk_mv_q8 (every format with integer codes); w, w2 2-byte aligned. Any tokens from 0
+ * to 2097120, any n from 1 to 2^30 (LK_ERANGE beyond). */
 int lk_mv_q8_ex(int fmt, int n, int k, int tokens, const uint8_t* xq, const void* w, const void* w2, const float* bias,
                 const float* bias2, int act, float alpha, float limit, const void* residual, int r_dtype, void* y,
                 int y_form, lk_stream_t stream);
@@ -214,9 +213,9 @@ int lk_gemm(int fmt, int mode, int rows, int k, int n, const uint16_t* x16, cons
  *   p[t][n] = scales[t][1] * sum_k x16[t][k] W16[n][k];  v = act(p + bias) or act(p + bias) * (p2 + bias2);  y = v + residual
  * W16: lk_gemm's f16 staging of every format it takes (one format for w and w2). The sums, bias, activation and residual
  * are f32; y is rounded once to y_dtype (LK_F32, LK_F16, LK_BF16). act, alpha, limit, biases and residual as lk_mv_q8_ex;
- * y may be the residual's buffer when both have the same type, and overlap no other operand. x16, scales as lk_gemm (x16 16-byte aligned), k % 64 == 0
- * and a whole number of the format's blocks; any rows >= 0 and any n from 1 to 2^30 (LK_ERANGE beyond); w, w2 2-byte
- * aligned (ggml MXFP4: any). */
+ * y may be the residual's buffer when both have the same type, and overlap no other operand (LK_EINVAL). x16, scales as
+ * lk_gemm (x16 16-byte aligned), k % 64 == 0 and a whole number of the format's blocks; any rows >= 0 and any n from 1 to
+ * 2^30 (LK_ERANGE beyond); w, w2 2-byte aligned (ggml MXFP4: any). */
 int lk_gemm_ex(int fmt, int rows, int k, int n, const uint16_t* x16, const float* scales, const void* w, const void* w2,
                const float* bias, const float* bias2, int act, float alpha, float limit, const void* residual,
                int r_dtype, void* y, int y_dtype, lk_stream_t stream);

@@ -12,10 +12,11 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 
 @pytest.fixture(scope="module")
 def walk(tmp_path_factory):
-    B.build()                                   # writes the table that the headers include
-    exe = str(tmp_path_factory.mktemp("walk") / "ring_walk")
+    tmp = str(tmp_path_factory.mktemp("walk"))
+    B._write_iq3s_grid(tmp)                     # the table that the formats' header includes
+    exe = os.path.join(tmp, "ring_walk")
     subprocess.check_call([B.NVCC, "-O2", "-std=c++17", "--expt-relaxed-constexpr", "-gencode",
-                           "arch=compute_100a,code=sm_100a", "-I", os.path.join(B.CSRC, "_build"), "-I", B.CSRC,
+                           "arch=compute_100a,code=sm_100a", "-I", tmp, "-I", B.CSRC,
                            os.path.join(HERE, "ring_walk.cu"), "-o", exe])
     return lambda *a: subprocess.run([exe, *a], capture_output=True, text=True, timeout=600)
 
